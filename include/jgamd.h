@@ -387,6 +387,36 @@ int32_t jgamd_dense_rows(const float *x1, const float *w1, int32_t K1, const flo
                          int32_t N, int32_t flags, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Product of rows with the weight of their type (nodes or edges sorted by
+ * type, rows sorted by expert):
+ *   out[r,:] = x[r,:] W[g] + bias[g]   for off[g] <= r < off[g+1], r in [0,M)
+ * and zero for rows of no type (before off[0], from off[G] on).  x [M][K],
+ * W [G][K][N], bias [G][N] or NULL, out [M][N], all of one `dtype`; sums in
+ * fp32.  JGAMD_WEIGHT_TRANSPOSED in `flags`: W is [G][N][K] (the input gradient
+ * dx = dout W^T is this call with dout for x and the forward's W).  off [G+1]
+ * stays on the device; offsets that fall or leave [0,M] are read as their
+ * running maximum clamped to [0,M].  Needs no workspace.
+ *
+ * jgamd_grouped_rows_weight_grad: dw[g] = sum over the rows of type g of
+ * x[r,:]^T dout[r,:] ([G][K][N]; zero for a type without rows) and, unless
+ * db is NULL, db[g] = sum of dout[r,:].  Fixed order, no atomics.
+ * No reference op: the reference has no typed product; its layers' x @ W
+ * (nn/conv/gcn_conv.py:95) is the case G = 1.
+ */
+#define JGAMD_F32 0
+#define JGAMD_BF16 1
+#define JGAMD_WEIGHT_TRANSPOSED 1
+int32_t jgamd_grouped_rows(const void *x, const void *w, const void *bias, const int32_t *off,
+                           void *out, int32_t M, int32_t K, int32_t N, int32_t G, int32_t dtype,
+                           int32_t flags, void *stream);
+int32_t jgamd_grouped_rows_weight_grad_workspace(int32_t M, int32_t K, int32_t N, int32_t G,
+                                                 size_t *bytes);
+int32_t jgamd_grouped_rows_weight_grad(const void *x, const void *dout, const int32_t *off,
+                                       void *dw, void *db, int32_t M, int32_t K, int32_t N,
+                                       int32_t G, int32_t dtype, void *ws, size_t ws_bytes,
+                                       void *stream);
+
+/* ------------------------------------------------------------------------
  * Column sums of a row-major [R,F] matrix: out[f] = sum_r x[r,f].  The bias
  * gradient of the conv layers (`out += self.bias`, nn/conv/gcn_conv.py:100-101,
  * nn/conv/sage_conv.py:189-190; Jittor derives the reduction).  Two stages,

@@ -58,6 +58,9 @@ SIGNATURES = {
     "jgamd_scatter_to_edge": [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _P],
     "jgamd_dense_rows_supported": [_I32, _I32, _I32],
     "jgamd_dense_rows": [_P, _P, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _P],
+    "jgamd_grouped_rows": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P],
+    "jgamd_grouped_rows_weight_grad_workspace": [_I32, _I32, _I32, _I32, _SZP],
+    "jgamd_grouped_rows_weight_grad": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _c.c_size_t, _P],
     "jgamd_column_sum_workspace": [_I64, _I32, _SZP],
     "jgamd_column_sum": [_P, _P, _I64, _I32, _P, _c.c_size_t, _P],
     "jgamd_relu_backward_column_sum": [_P, _P, _P, _P, _I64, _I32, _P, _c.c_size_t, _P],
@@ -112,6 +115,36 @@ def ptr(t):
 
 def stream_ptr(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on:
+    """Makes `device` the current one for a launch (a stream belongs to its device); free where it
+    already is."""
+
+    def __init__(self, device):
+        self._guard = None
+        if device.index is not None and device.index != torch.cuda.current_device():
+            self._guard = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+        return False
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}      # JGAMD_F32, JGAMD_BF16
+
+
+def dtype_code(dtype):
+    """The header's number of an element type; an error for one the kernels do not take."""
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise JgamdError("the kernels take float32 or bfloat16, got %s" % dtype)
+    return code
 
 
 def require_gpu(*tensors):
