@@ -417,6 +417,34 @@ int32_t jgamd_grouped_rows_weight_grad(const void *x, const void *dout, const in
                                        void *stream);
 
 /* ------------------------------------------------------------------------
+ * The end of a residual block, row by row of [R][F] (F <= 8192):
+ *   ry = (mean_f y^2 + eps)^-1/2
+ *   s  = x + scale[f] sigmoid(gate) (y ry post[f])
+ *   rs = (mean_f s^2 + eps)^-1/2,   h = s rs w[f]
+ * gate [R][F], scale [F], post [F] may each be NULL (a factor of 1; without
+ * post y is not normalised either), and so may y (s = x: the first norm of a
+ * network; s is then not written), s (not written) and ry, rs ([R] each, what
+ * the backward call wants).  All arrays but ry, rs are of one `dtype`
+ * (JGAMD_F32 / JGAMD_BF16); arithmetic is fp32.
+ *
+ * jgamd_residual_norm_bwd: the gradients from ds, dh ([R][F], NULL = zero)
+ * and the forward's inputs and ry, rs.  Every output may be NULL.  dscale,
+ * dpost, dw are sums over the rows in a fixed order, no atomics; only they
+ * need the workspace.  No reference op: the reference's layers have no norms;
+ * GCN2Conv's initial residual (nn/conv/gcn2_conv.py:70-73) is the nearest.
+ */
+int32_t jgamd_residual_norm_fwd(const void *x, const void *y, const void *gate, const void *scale,
+                                const void *post, const void *w, void *s, void *h, float *ry,
+                                float *rs, int64_t R, int32_t F, float eps, int32_t dtype,
+                                void *stream);
+int32_t jgamd_residual_norm_bwd_workspace(int64_t R, int32_t F, size_t *bytes);
+int32_t jgamd_residual_norm_bwd(const void *x, const void *y, const void *gate, const void *scale,
+                                const void *post, const void *w, const float *ry, const float *rs,
+                                const void *ds, const void *dh, void *dx, void *dy, void *dgate,
+                                void *dscale, void *dpost, void *dw, int64_t R, int32_t F,
+                                int32_t dtype, void *ws, size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
  * Column sums of a row-major [R,F] matrix: out[f] = sum_r x[r,f].  The bias
  * gradient of the conv layers (`out += self.bias`, nn/conv/gcn_conv.py:100-101,
  * nn/conv/sage_conv.py:189-190; Jittor derives the reduction).  Two stages,

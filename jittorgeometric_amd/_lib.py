@@ -61,6 +61,10 @@ SIGNATURES = {
     "jgamd_grouped_rows": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P],
     "jgamd_grouped_rows_weight_grad_workspace": [_I32, _I32, _I32, _I32, _SZP],
     "jgamd_grouped_rows_weight_grad": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _c.c_size_t, _P],
+    "jgamd_residual_norm_fwd": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _F32, _I32, _P],
+    "jgamd_residual_norm_bwd_workspace": [_I64, _I32, _SZP],
+    "jgamd_residual_norm_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P,
+                                _c.c_size_t, _P],
     "jgamd_column_sum_workspace": [_I64, _I32, _SZP],
     "jgamd_column_sum": [_P, _P, _I64, _I32, _P, _c.c_size_t, _P],
     "jgamd_relu_backward_column_sum": [_P, _P, _P, _P, _I64, _I32, _P, _c.c_size_t, _P],

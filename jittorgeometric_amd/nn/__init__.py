@@ -2,3 +2,4 @@ from .conv import (APPNP, BernNet, ChebConv, ChebNetII, ClusterGCNConv, EvenNet,
                    MessagePassingNts, SAGEConv, SGConv, clustergcn_norm, gcn_norm, sage_norm)
 from .loss import cross_entropy_loss, nll_loss  # noqa: F401
 from .typed import TypedLinear  # noqa: F401
+from .norm import residual_norm, rms_norm  # noqa: F401

@@ -59,3 +59,46 @@ def test_wrappers_refuse_cpu_tensors():
     from jittorgeometric_amd.ops import grouped_rows
     with pytest.raises(JgamdError):
         grouped_rows(torch.zeros(4, 3), torch.zeros(2, 3, 5), torch.zeros(3, dtype=torch.int32))
+
+
+def test_residual_norm_arguments(lib):
+    n = ctypes.c_size_t(0)
+    fwd, bwd = lib.jgamd_residual_norm_fwd, lib.jgamd_residual_norm_bwd
+    for R, F in ((-1, 8), (5, 0), (5, 8193), (1 << 31, 8)):
+        assert fwd(*[BAD] * 10, R, F, 1e-6, 0, None) == -2
+        assert bwd(*[BAD] * 16, R, F, 0, BAD, 1 << 40, None) == -2
+        assert lib.jgamd_residual_norm_bwd_workspace(R, F, ctypes.byref(n)) == -2
+    assert lib.jgamd_residual_norm_bwd_workspace(5, 8, None) == -1
+    assert fwd(*[BAD] * 10, 5, 8, 1e-6, 3, None) == -4
+    assert bwd(*[BAD] * 16, 5, 8, 3, BAD, 1 << 40, None) == -4
+    for i in (0, 5, 7):                                        # x, w, h
+        args = [BAD] * 10
+        args[i] = None
+        assert fwd(*args, 5, 8, 1e-6, 0, None) == -1
+    assert fwd(BAD, None, BAD, None, None, BAD, None, BAD, None, None, 5, 8, 1e-6, 0, None) == -1      # gate without y
+    for i in range(10):
+        args = [BAD] * 10
+        args[i] = ODD
+        assert fwd(*args, 5, 8, 1e-6, 1, None) == -5
+    assert fwd(*[None] * 10, 0, 8, 1e-6, 0, None) == 0
+    assert lib.jgamd_residual_norm_bwd_workspace(100_000, 256, ctypes.byref(n)) == 0 and 0 < n.value < 1 << 24
+    for i in (0, 1, 2, 3, 4, 5, 6, 7):                         # an input that a gradient needs
+        args = [BAD] * 16
+        args[i] = None
+        assert bwd(*args, 5, 8, 0, BAD, 1 << 40, None) == -1
+    for i in range(16):
+        args = [BAD] * 16
+        args[i] = ODD
+        assert bwd(*args, 5, 8, 1, BAD, 1 << 40, None) == -5
+    assert bwd(*[BAD] * 16, 5, 8, 0, None, 0, None) == -3
+    assert bwd(*[BAD] * 16, 5, 8, 0, BAD, 16, None) == -3
+    assert bwd(*[BAD] * 16, 5, 8, 0, ctypes.c_void_p(260), 1 << 40, None) == -5
+
+
+def test_norm_wrappers_refuse_cpu_tensors():
+    from jittorgeometric_amd import JgamdError
+    from jittorgeometric_amd.nn import residual_norm, rms_norm
+    with pytest.raises(JgamdError):
+        rms_norm(torch.zeros(4, 3), torch.ones(3))
+    with pytest.raises(JgamdError):
+        residual_norm(torch.zeros(4, 3), torch.zeros(4, 3), torch.ones(3))
