@@ -387,6 +387,41 @@ int32_t jgamd_dense_rows(const float *x1, const float *w1, int32_t K1, const flo
                          int32_t N, int32_t flags, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Softmax cross entropy of z = x w^T + bias without the [V][C] logits:
+ *   lse[i]  = log sum_c exp(z[i,c])
+ *   loss[i] = lse[i] - z[i,label[i]], 0 for labels outside [0,C)
+ * x [V][F], w [C][F] (a row per class), bias [C] or NULL, all of `dtype`
+ * (JGAMD_F32 / JGAMD_BF16; JGAMD_F32 = 0, JGAMD_BF16 = 1 below); sums, lse and
+ * loss fp32.  `reduction`: JGAMD_LOSS_MEAN over the rows with a label (NaN when
+ * there is none) and JGAMD_LOSS_SUM write loss[0] and count[0] = those rows,
+ * JGAMD_LOSS_NONE writes loss[V] (count is not written).
+ *
+ * jgamd_linear_cross_entropy_bwd: dx [V][F], dw [C][F], db [C] (each may be
+ * NULL; db needs dw) from grad ([1], or [V] with JGAMD_LOSS_NONE) and the
+ * forward's lse and count.  The workspace (the query with backward = 1) holds
+ * the gradient of the logits for a block of rows and a piece of the classes,
+ * at most 2^27 numbers, and fp32 sums.  Fixed order, no atomics.
+ * With few classes: jgamd_cross_entropy_fwd / _bwd on logits
+ * (nn.cross_entropy_loss(pred, label), examples/gcn_example.py:113).
+ */
+#define JGAMD_LOSS_NONE 0
+#define JGAMD_LOSS_MEAN 1
+#define JGAMD_LOSS_SUM 2
+int32_t jgamd_linear_cross_entropy_workspace(int64_t V, int32_t F, int32_t C, int32_t dtype,
+                                             int32_t backward, size_t *bytes);
+int32_t jgamd_linear_cross_entropy_fwd(const void *x, const void *w, const void *bias,
+                                       const void *labels, int32_t labels_are_i64, int64_t V,
+                                       int32_t F, int32_t C, int32_t dtype, int32_t reduction,
+                                       float *loss, int32_t *count, float *lse, void *ws,
+                                       size_t ws_bytes, void *stream);
+int32_t jgamd_linear_cross_entropy_bwd(const void *x, const void *w, const void *bias,
+                                       const void *labels, int32_t labels_are_i64,
+                                       const float *lse, const int32_t *count, const float *grad,
+                                       int64_t V, int32_t F, int32_t C, int32_t dtype,
+                                       int32_t reduction, void *dx, void *dw, void *db, void *ws,
+                                       size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
  * Product of rows with the weight of their type (nodes or edges sorted by
  * type, rows sorted by expert):
  *   out[r,:] = x[r,:] W[g] + bias[g]   for off[g] <= r < off[g+1], r in [0,M)

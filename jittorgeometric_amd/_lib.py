@@ -58,6 +58,11 @@ SIGNATURES = {
     "jgamd_scatter_to_edge": [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _P],
     "jgamd_dense_rows_supported": [_I32, _I32, _I32],
     "jgamd_dense_rows": [_P, _P, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _P],
+    "jgamd_linear_cross_entropy_workspace": [_I64, _I32, _I32, _I32, _I32, _SZP],
+    "jgamd_linear_cross_entropy_fwd": [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _c.c_size_t,
+                                       _P],
+    "jgamd_linear_cross_entropy_bwd": [_P, _P, _P, _P, _I32, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P,
+                                       _c.c_size_t, _P],
     "jgamd_grouped_rows": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P],
     "jgamd_grouped_rows_weight_grad_workspace": [_I32, _I32, _I32, _I32, _SZP],
     "jgamd_grouped_rows_weight_grad": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _c.c_size_t, _P],

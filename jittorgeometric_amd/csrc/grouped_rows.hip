@@ -194,7 +194,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads) void
     const Operand<T> p{static_cast<const T *>(a.dout) + (int64_t)row0 * a.N + n0, a.N, a.N - n0};
     const Operand<T> q{static_cast<const T *>(a.x) + (int64_t)row0 * a.K + k0, a.K, a.K - k0};
     const bool with_bias = a.db && k0 == 0;
-    if (with_bias) Product::template run<true>(acc, p, q, 0, rows, lds, sums);
+    if (with_bias) Product::template run<kSumP>(acc, p, q, 0, rows, lds, sums);
     else Product::run(acc, p, q, 0, rows, lds);
 
     const bool direct = run.pieces == 1;

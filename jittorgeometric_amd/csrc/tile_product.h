@@ -35,6 +35,7 @@ struct bf16 {      // storage only
 };
 
 enum Layout { kAlongK, kAcrossK };
+enum Sums { kNoSums, kSumP, kSumQ };
 
 // two floats, rounded to nearest even, as two bfloat16 in one register
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b)
@@ -225,9 +226,11 @@ template <typename T, typename S, Layout PL, Layout QL> struct TileProduct {
     static constexpr int kLds = StageP::kBytes + StageQ::kBytes;
     static constexpr int kParts = Eight<T>::kParts;
 
-    // acc += products over k_beg .. k_end - 1.  With ROWSUM, sums[i] += sum_k P[n][k] as well.
+    // acc += products over k_beg .. k_end - 1.  SUMS: also the sums of one operand over k, as products
+    // with ones: kSumP: sums[i] += sum_k P[n][k] in every lane, at the registers of n; kSumQ:
+    // sums[j] += sum_k Q[m][k] in every register, at the lanes of m.
     // Every wavefront of the workgroup calls it, with the same arguments.
-    template <bool ROWSUM = false>
+    template <Sums SUMS = kNoSums>
     __device__ __forceinline__ static void run(f32x4 (&acc)[S::FN][S::FM], const Operand<T> &p, const Operand<T> &q,
                                                int k_beg, int k_end, char *lds, f32x4 *sums = nullptr)
     {
@@ -270,15 +273,20 @@ template <typename T, typename S, Layout PL, Layout QL> struct TileProduct {
                             for (int j = 0; j < S::FM; j++)
                                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[a][i], fq[sum - a][j], acc[i][j],
                                                                                     0, 0, 0);
-                if (ROWSUM) {
-                    const uint32_t one = 0x3f803f80u;
-                    const u32x4 ones = {one, one, one, one};
+                if (SUMS != kNoSums) {
+                    const uint32_t one = 0x3f803f80u;      // two bfloat16 ones
+                    const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one, one, one, one});
 #pragma unroll
-                    for (int s = kParts - 1; s >= 0; s--)
+                    for (int s = kParts - 1; s >= 0; s--) {
+                        if (SUMS == kSumP)
 #pragma unroll
-                        for (int i = 0; i < S::FN; i++)
-                            sums[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                fp[s][i], __builtin_bit_cast(bf16x8, ones), sums[i], 0, 0, 0);
+                            for (int i = 0; i < S::FN; i++)
+                                sums[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[s][i], ones, sums[i], 0, 0, 0);
+                        else
+#pragma unroll
+                            for (int j = 0; j < S::FM; j++)
+                                sums[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fq[s][j], sums[j], 0, 0, 0);
+                    }
                 }
             }
         }

@@ -3,8 +3,10 @@ training steps (nn.cross_entropy_loss(pred, label) in examples/gcn_example.py:11
 nn.log_softmax + nn.nll_loss in examples/sage_example.py:69,83; both functions live in
 the jittor package).  Forward and gradient are one library kernel each
 (csrc/loss.hip): with millions of rows and a few dozen classes a generic framework
-loss spends most of its time in single-block reductions."""
+loss spends most of its time in single-block reductions.  linear_cross_entropy is the same
+loss behind a linear map onto many classes, without the logits (csrc/class_head.hip)."""
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -64,3 +66,86 @@ def nll_loss(log_probs, target):
     log_softmax + nll_loss, examples/sage_example.py:69,83); the gradient is -1 / rows at the
     labels and zero elsewhere.  Same kernels, with the softmax term switched off."""
     return _CrossEntropy.apply(log_probs, target, True)
+
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}      # JGAMD_LOSS_NONE, JGAMD_LOSS_MEAN, JGAMD_LOSS_SUM
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, reduction):
+        lib = _lib.load()
+        dev = x.device
+        V, F = x.shape
+        C = weight.shape[0]
+        code = _lib.dtype_code(x.dtype)
+        i64 = 1 if target.dtype == torch.int64 else 0
+        loss = torch.empty((V,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+        count = torch.empty((), dtype=torch.int32, device=dev)
+        lse = torch.empty(V, dtype=torch.float32, device=dev)
+        nbytes = _lib.query(lib.jgamd_linear_cross_entropy_workspace, V, F, C, code, 0)
+        ws = _lib.workspace(nbytes, dev)
+        with _lib.on(dev):
+            _lib.check(lib.jgamd_linear_cross_entropy_fwd(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(target),
+                                                          i64, V, F, C, code, reduction, _lib.ptr(loss), _lib.ptr(count),
+                                                          _lib.ptr(lse), _lib.ptr(ws), nbytes, _lib.stream_ptr(dev)))
+        ctx.save_for_backward(x, weight, bias, target, lse, count)
+        ctx.reduction = reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, bias, target, lse, count = ctx.saved_tensors
+        lib = _lib.load()
+        dev = x.device
+        V, F = x.shape
+        C = weight.shape[0]
+        code = _lib.dtype_code(x.dtype)
+        g = g.to(torch.float32).contiguous()
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else None
+        db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
+        nbytes = _lib.query(lib.jgamd_linear_cross_entropy_workspace, V, F, C, code, 1)
+        ws = _lib.workspace(nbytes, dev)
+        with _lib.on(dev):
+            _lib.check(lib.jgamd_linear_cross_entropy_bwd(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(target),
+                                                          1 if target.dtype == torch.int64 else 0, _lib.ptr(lse),
+                                                          _lib.ptr(count), _lib.ptr(g), V, F, C, code, ctx.reduction,
+                                                          _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), nbytes,
+                                                          _lib.stream_ptr(dev)))
+        return dx, dw, db, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
+    """cross_entropy_loss(x @ weight.t() + bias, target) without the [rows, classes] logits, in memory
+    or in the workspace: for classes by the ten thousand (items, entities, words).
+
+    x [rows, features], weight [classes, features] (a row per class, as an embedding table), bias
+    [classes] or None, all float32 or all bfloat16; target [rows], int32 or int64.  Rows whose label
+    lies outside [0, classes) are left out of the mean, have loss 0 and get a zero gradient.
+    reduction: "mean" over the rows with a label (NaN when there is none), "sum" or "none" ([rows]);
+    the loss is float32.  A class may be masked with a bias of -inf.  Products are summed in float32;
+    a float32 product keeps float32's 24 bits, but an entry of x or weight of 3.39e38 or more, an
+    infinity or a NaN makes the logits it enters NaN.  The gradient of the logits is rounded to the
+    type of x on its way into the gradients of x, weight and bias."""
+    _lib.require_gpu(x, weight, target, bias)
+    if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
+        raise _lib.JgamdError("linear_cross_entropy: x must be [rows, features] and weight [classes, features], got %s "
+                              "and %s" % (tuple(x.shape), tuple(weight.shape)))
+    if 0 in weight.shape:
+        raise _lib.JgamdError("linear_cross_entropy: weight has no elements: %s" % (tuple(weight.shape),))
+    if target.dim() != 1 or target.shape[0] != x.shape[0]:
+        raise _lib.JgamdError("linear_cross_entropy: %d labels for %d rows" % (target.numel(), x.shape[0]))
+    if target.dtype not in (torch.int32, torch.int64):
+        raise _lib.JgamdError("linear_cross_entropy: labels must be int32 or int64, got %s" % target.dtype)
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise _lib.JgamdError("linear_cross_entropy: bias must be [%d], got %s" % (weight.shape[0], tuple(bias.shape)))
+    if reduction not in _REDUCTIONS:
+        raise _lib.JgamdError("linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
+    _lib.dtype_code(x.dtype)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype != x.dtype:
+            raise _lib.JgamdError("linear_cross_entropy: %s is %s, x is %s" % (name, t.dtype, x.dtype))
+    return _LinearCrossEntropy.apply(x.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(),
+                                     target.contiguous(), _REDUCTIONS[reduction])

@@ -102,3 +102,40 @@ def test_norm_wrappers_refuse_cpu_tensors():
         rms_norm(torch.zeros(4, 3), torch.ones(3))
     with pytest.raises(JgamdError):
         residual_norm(torch.zeros(4, 3), torch.zeros(4, 3), torch.ones(3))
+
+
+def test_linear_cross_entropy_arguments(lib):
+    n = ctypes.c_size_t(0)
+    fwd, bwd, size = (lib.jgamd_linear_cross_entropy_fwd, lib.jgamd_linear_cross_entropy_bwd,
+                      lib.jgamd_linear_cross_entropy_workspace)
+    for V, F, C in ((-1, 8, 9), (5, 0, 9), (5, 8, 0), (1 << 31, 8, 9), (5, (1 << 20) + 1, 9), (5, 8, 2**31 - 1)):
+        assert size(V, F, C, 0, 0, ctypes.byref(n)) == -2
+        assert fwd(*[BAD] * 4, 1, V, F, C, 0, 1, *[BAD] * 4, 1 << 40, None) == -2
+        assert bwd(*[BAD] * 4, 1, *[BAD] * 3, V, F, C, 0, 1, *[BAD] * 4, 1 << 40, None) == -2
+    assert size(5, 8, 9, 0, 0, None) == -1
+    assert size(5, 8, 9, 2, 0, ctypes.byref(n)) == -4
+    assert fwd(*[BAD] * 4, 1, 5, 8, 9, 0, 3, *[BAD] * 4, 1 << 40, None) == -2
+    assert fwd(*[BAD] * 4, 1, 5, 8, 9, 2, 1, *[BAD] * 4, 1 << 40, None) == -4
+    for i in (0, 1, 3, 9, 10, 11):                      # x, w, labels; loss, count, lse
+        a = [BAD] * 4 + [1, 5, 8, 9, 0] + [BAD] * 3
+        a[i] = None
+        assert fwd(*a[:9], 1, *a[9:], BAD, 1 << 40, None) == -1
+        if i < 4:
+            assert bwd(*a[:4], 1, *[BAD] * 3, 5, 8, 9, 0, 1, *[BAD] * 4, 1 << 40, None) == -1
+    for i in range(4):
+        a = [BAD] * 4
+        a[i] = ODD
+        assert fwd(*a, 1, 5, 8, 9, 1, 1, *[BAD] * 4, 1 << 40, None) == -5
+        assert bwd(*a, 1, *[BAD] * 3, 5, 8, 9, 1, 1, *[BAD] * 4, 1 << 40, None) == -5
+    assert fwd(*[BAD] * 4, 1, 5, 8, 9, 0, 1, *[BAD] * 3, None, 0, None) == -3
+    assert fwd(*[BAD] * 4, 1, 5, 8, 9, 0, 1, *[BAD] * 4, 16, None) == -3
+    assert fwd(*[BAD] * 4, 1, 5, 8, 9, 0, 1, *[BAD] * 3, ctypes.c_void_p(260), 1 << 40, None) == -5
+    assert bwd(*[BAD] * 4, 1, *[BAD] * 3, 5, 8, 9, 0, 1, BAD, None, BAD, BAD, 1 << 40, None) == -1      # db without dw
+    assert bwd(*[BAD] * 4, 1, *[BAD] * 3, 5, 8, 9, 0, 1, *[BAD] * 3, None, 0, None) == -3
+    assert bwd(*[BAD] * 4, 1, *[BAD] * 3, 5, 8, 9, 0, 1, *[BAD] * 4, 16, None) == -3
+    assert bwd(*[BAD] * 4, 1, *[BAD] * 3, 5, 8, 9, 0, 1, None, None, None, None, 0, None) == 0
+    for back in (0, 1):
+        assert size(0, 8, 9, 0, back, ctypes.byref(n)) == 0
+    # the scratch does not grow with rows * classes
+    assert size(1 << 20, 256, 1 << 20, 1, 1, ctypes.byref(n)) == 0 and n.value < 3 << 30
+    assert size(1 << 20, 256, 1 << 20, 1, 0, ctypes.byref(n)) == 0 and n.value < 1 << 30
