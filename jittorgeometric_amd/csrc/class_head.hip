@@ -16,18 +16,36 @@
 //
 // Bound by the matrix units from some hundred rows on, by reading w below that.
 #include <algorithm>
+#include <mutex>
 
-#include "tile_product.h"
+#include "stream_product.h"
 
 namespace jg {
 
 constexpr int kHeadMaxFeatures = 1 << 20;
-constexpr int64_t kPieceElements = (int64_t)1 << 27;
+constexpr int64_t kPieceElements = (int64_t)1 << 28;
 constexpr int kBlockRows = 16384;      // rows of a block of the backward pass
 constexpr int kJoinThreads = 256;
+constexpr int kCus = 256;
+constexpr int kPad = 128;      // classes between the rows of d: rows a power of two apart meet in one channel of the L2
+
+// bfloat16: 256 x 128 results, four wavefronts of 128 x 64, three stages (72 KB of LDS): two workgroups
+// a compute unit, one of which multiplies while the other writes its results.
+// float: three parts an operand, 256 x 128 results, two stages (144 KB).
+template <typename T> struct HeadShapeOf;
+template <> struct HeadShapeOf<bf16> {
+    using S = StreamShape<1, 256, 128, 2, 2, 3>;
+};
+template <> struct HeadShapeOf<float> {
+    using S = StreamShape<3, 256, 128, 4, 2, 2>;
+};
+template <typename T> using HeadShape = typename HeadShapeOf<T>::S;
 
 struct HeadArgs {
-    const void *x, *w, *bias;
+    const bf16 *x, *w;           // [V][ld], [C][ld] as parts (stream_product.h)
+    int64_t part_x, part_w;
+    int ld;                      // F rounded up to 8
+    const void *bias;            // [C] of T, or NULL
     const int32_t *y32;
     const int64_t *y64;
     int64_t V;
@@ -61,73 +79,124 @@ template <typename T> __device__ __forceinline__ f32x4 bias4(const void *bias, i
     return b;
 }
 
-// grid: x = blocks of BM rows x ranges of class tiles, ranges fastest.  stats [ranges][V]
+// Order of the tiles of an M x N grid of tiles: runs of consecutive numbers cover blocks of up to 8 x 4
+// tiles, and the workgroups of one XCD (every eighth) work on one run, so that the operands of a run
+// are read into one L2 once.  `step` counts the tiles of workgroup blockIdx.x.
+__device__ __forceinline__ void tile_at(int step, int mtiles, int ntiles, int *m, int *n, bool *exists)
+{
+    const int g = gridDim.x, b = blockIdx.x;
+    const int64_t id = (int64_t)step * g + (g % 8 == 0 ? (b % 8) * (g / 8) + b / 8 : b);
+    *exists = id < (int64_t)mtiles * ntiles;
+    const int64_t group = id / ((int64_t)8 * ntiles);
+    const int height = min(8, mtiles - (int)group * 8);
+    const int in = (int)(id - group * 8 * ntiles);
+    *m = (int)group * 8 + in % max(height, 1);
+    *n = in / max(height, 1);
+}
+// how many tiles workgroup blockIdx.x has
+__device__ __forceinline__ int tiles_of(int mtiles, int ntiles)
+{
+    const int g = gridDim.x, b = blockIdx.x;
+    const int64_t all = (int64_t)mtiles * ntiles;
+    const int64_t first = g % 8 == 0 ? (b % 8) * (g / 8) + b / 8 : b;
+    return first < all ? (int)((all - 1 - first) / g + 1) : 0;
+}
+
+// Parts of an array: [R][F] of T to PARTS arrays [R][ld] of bfloat16, zero behind F.
+// grid: x = pieces of 8
+template <typename T>
+__global__ __launch_bounds__(256) void head_parts(const T *__restrict__ src, int64_t R, int F, int ld, bf16 *__restrict__ dst,
+                                                  int64_t part)
+{
+    const int across = ld / 8;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= R * across) return;
+    const int64_t row = id / across;
+    const int c = (int)(id - row * across) * 8;
+    Eight<T> e;
+    if (c + 8 <= F) e.load(src + row * F + c);
+    else e.load_some(src + row * F + c, F - c);
+    e.store_parts(dst + row * ld + c, part);
+}
+
+// grid: x = blocks of BM rows x ranges of class tiles.  stats [ranges][V]
 template <typename T, typename S>
-__global__ __launch_bounds__(S::kThreads) void head_stats(HeadArgs a, int ranges, int tiles_per_range,
+__global__ __launch_bounds__(S::kThreads, 2) void head_stats(HeadArgs a, int ranges, int tiles_per_range,
                                                           float2 *__restrict__ stats, float *__restrict__ at_label)
 {
-    using Product = TileProduct<T, S, kAlongK, kAlongK>;
-    __shared__ __align__(16) char lds[Product::kLds];
-    __shared__ float2 joined[S::WN][S::BM];
-    const int range = blockIdx.x % ranges;
-    const int64_t row0 = (int64_t)(blockIdx.x / ranges) * S::BM;
+    using Product = StreamProduct<S, kAlongK, kAlongK>;
+    extern __shared__ __align__(16) char lds[];
+    const int blocks = (int)((a.V + S::BM - 1) / S::BM);
+    int block, range;
+    bool exists;
+    tile_at(0, blocks, ranges, &block, &range, &exists);
+    if (!exists) return;
+    const int64_t row0 = (int64_t)block * S::BM;
     const int rows = (int)min((int64_t)S::BM, a.V - row0);
-    const Operand<T> q{static_cast<const T *>(a.x) + row0 * a.F, a.F, rows};
     float m[S::FM], s[S::FM];
     int label[S::FM];
 #pragma unroll
     for (int j = 0; j < S::FM; j++) {
         m[j] = -INFINITY;
         s[j] = 0.f;
-        label[j] = m_of<S>(j) < rows ? (int)head_label(a, row0 + m_of<S>(j)) : -1;
+        label[j] = Product::m_of(j) < rows ? (int)head_label(a, row0 + Product::m_of(j)) : -1;
     }
     const int tiles = (a.C + S::BN - 1) / S::BN;
-    const int last = min(tiles, (range + 1) * tiles_per_range);
-    for (int tile = range * tiles_per_range; tile < last; tile++) {
-        const int c0 = tile * S::BN;
-        f32x4 acc[S::FN][S::FM];
+    const int first = range * tiles_per_range;
+    const bf16 *x = a.x + row0 * a.ld;
+    Product::template run<kNoSums>(
+        min(tiles, first + tiles_per_range) - first, lds,
+        [&](int t) {
+            const int c0 = (first + t) * S::BN;
+            return StreamTile{a.w + (int64_t)c0 * a.ld, x, a.part_w, a.part_x, a.ld, a.ld, a.C - c0, rows, a.F};
+        },
+        [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *) {
+            const int c0 = (first + t) * S::BN;
+            if (a.bias) {
 #pragma unroll
-        for (int i = 0; i < S::FN; i++) {
-            const f32x4 b = bias4<T>(a.bias, c0 + n_of<S>(i), a.C);
+                for (int i = 0; i < S::FN; i++) {
+                    const f32x4 b = bias4<T>(a.bias, c0 + Product::n_of(i), a.C);
 #pragma unroll
-            for (int j = 0; j < S::FM; j++) acc[i][j] = b;
-        }
-        const Operand<T> p{static_cast<const T *>(a.w) + (int64_t)c0 * a.F, a.F, a.C - c0};
-        Product::run(acc, p, q, 0, a.F, lds);
-        if (c0 + S::BN > a.C) {      // classes past the last count as -inf
+                    for (int j = 0; j < S::FM; j++) acc[i][j] += b;
+                }
+            }
+            if (c0 + S::BN > a.C) {      // classes past the last count as -inf
 #pragma unroll
-            for (int i = 0; i < S::FN; i++)
+                for (int i = 0; i < S::FN; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (c0 + n_of<S>(i) + r >= a.C)
+                    for (int r = 0; r < 4; r++)
+                        if (c0 + Product::n_of(i) + r >= a.C)
 #pragma unroll
-                        for (int j = 0; j < S::FM; j++) acc[i][j][r] = -INFINITY;
-        }
+                            for (int j = 0; j < S::FM; j++) acc[i][j][r] = -INFINITY;
+            }
 #pragma unroll
-        for (int j = 0; j < S::FM; j++) {
-            float top = m[j];
+            for (int j = 0; j < S::FM; j++) {
+                float top = m[j];
 #pragma unroll
-            for (int i = 0; i < S::FN; i++)
+                for (int i = 0; i < S::FN; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) top = fmaxf(top, acc[i][j][r]);
-            const float ref = top == -INFINITY ? 0.f : top;
-            float sum = s[j] * __expf(m[j] - ref);
+                    for (int r = 0; r < 4; r++) top = fmaxf(top, acc[i][j][r]);
+                const float ref = top == -INFINITY ? 0.f : top;
+                float sum = s[j] * __expf(m[j] - ref);
 #pragma unroll
-            for (int i = 0; i < S::FN; i++)
+                for (int i = 0; i < S::FN; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) sum += __expf(acc[i][j][r] - ref);
-            m[j] = top;
-            s[j] = sum;
-            // the one lane that holds the label's logit hands it on
-            const int at = label[j] - c0;
+                    for (int r = 0; r < 4; r++) sum += __expf(acc[i][j][r] - ref);
+                m[j] = top;
+                s[j] = sum;
+                // the one lane that holds the label's logit hands it on
+                const int at = label[j] - c0;
+                if (at >= 0 && at < S::BN) {
 #pragma unroll
-            for (int i = 0; i < S::FN; i++)
+                    for (int i = 0; i < S::FN; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (at == n_of<S>(i) + r) at_label[row0 + m_of<S>(j)] = acc[i][j][r];
-        }
-    }
+                        for (int r = 0; r < 4; r++)
+                            if (at == Product::n_of(i) + r) at_label[row0 + Product::m_of(j)] = acc[i][j][r];
+                }
+            }
+        });
     // the four lanes of a row, then the wavefronts beside each other
+    float2 *joined = reinterpret_cast<float2 *>(lds);      // [WN][BM]
 #pragma unroll
     for (int j = 0; j < S::FM; j++) {
 #pragma unroll
@@ -135,34 +204,46 @@ __global__ __launch_bounds__(S::kThreads) void head_stats(HeadArgs a, int ranges
             const float m2 = __shfl_xor(m[j], o, kWave), s2 = __shfl_xor(s[j], o, kWave);
             join_stats(m[j], s[j], m2, s2);
         }
-        if (lane_id() < 16) joined[wave_in_block() / S::WM][m_of<S>(j)] = float2{m[j], s[j]};
+        if (lane_id() < 16) joined[(wave_in_block() / S::WM) * S::BM + Product::m_of(j)] = float2{m[j], s[j]};
     }
     __syncthreads();
     for (int r = threadIdx.x; r < rows; r += S::kThreads) {
-        float2 v = joined[0][r];
+        float2 v = joined[r];
 #pragma unroll
-        for (int k = 1; k < S::WN; k++) join_stats(v.x, v.y, joined[k][r].x, joined[k][r].y);
+        for (int k = 1; k < S::WN; k++) join_stats(v.x, v.y, joined[k * S::BM + r].x, joined[k * S::BM + r].y);
         stats[(int64_t)range * a.V + row0 + r] = v;
     }
 }
 
-// a row's ranges joined: lse, loss; and the workgroup's sum of losses and number of labels
-__global__ __launch_bounds__(kJoinThreads) void head_rows(HeadArgs a, int ranges, const float2 *__restrict__ stats,
+// Joins a row's ranges to lse and loss, `lanes` lanes a row (a power of two up to 64), and adds the
+// workgroup's losses and labels in a fixed order; with one workgroup that is the result.
+// grid: x = rows / (kJoinThreads / lanes)
+__global__ __launch_bounds__(kJoinThreads) void head_rows(HeadArgs a, int ranges, int lanes, int mean,
+                                                          const float2 *__restrict__ stats,
                                                           const float *__restrict__ at_label, float *__restrict__ lse,
                                                           float *__restrict__ row_loss, double *__restrict__ block_sum,
-                                                          int32_t *__restrict__ block_count)
+                                                          int32_t *__restrict__ block_count, float *__restrict__ total,
+                                                          int32_t *__restrict__ total_count)
 {
     __shared__ double s_sum[kJoinThreads / kWave];
     __shared__ int s_count[kJoinThreads / kWave];
-    const int64_t row = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;
-    double loss = 0.0;
-    int count = 0;
+    const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / lanes) + threadIdx.x / lanes;
+    const int lane = threadIdx.x % lanes;
+    float m = -INFINITY, s = 0.f;
     if (row < a.V) {
-        float m = -INFINITY, s = 0.f;
-        for (int k = 0; k < ranges; k++) {
+#pragma unroll 4
+        for (int k = lane; k < ranges; k += lanes) {
             const float2 v = stats[(int64_t)k * a.V + row];
             join_stats(m, s, v.x, v.y);
         }
+    }
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor(m, o, kWave), s2 = __shfl_xor(s, o, kWave);
+        join_stats(m, s, m2, s2);
+    }
+    double loss = 0.0;
+    int count = 0;
+    if (row < a.V && lane == 0) {
         const float l = m + logf(s);
         lse[row] = l;
         const bool counted = head_label(a, row) >= 0;
@@ -171,6 +252,7 @@ __global__ __launch_bounds__(kJoinThreads) void head_rows(HeadArgs a, int ranges
         loss = (double)v;
         count = counted ? 1 : 0;
     }
+    if (row_loss) return;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         loss += __shfl_xor(loss, o, kWave);
@@ -186,8 +268,13 @@ __global__ __launch_bounds__(kJoinThreads) void head_rows(HeadArgs a, int ranges
             loss += s_sum[k];
             count += s_count[k];
         }
-        block_sum[blockIdx.x] = loss;
-        block_count[blockIdx.x] = count;
+        if (gridDim.x == 1) {
+            total[0] = (float)(mean ? loss / (double)count : loss);
+            total_count[0] = count;
+        } else {
+            block_sum[blockIdx.x] = loss;
+            block_count[blockIdx.x] = count;
+        }
     }
 }
 
@@ -227,54 +314,108 @@ struct PieceArgs {
     int per_row;
     int64_t row0;              // the block of rows and the piece of classes
     int rows, c0, classes;
-    void *d;                   // [rows][ld]
-    int64_t ld;
+    bf16 *d;                   // [rows][ld] as parts
+    int64_t part;
+    int ld;
 };
 
-// d for a block of rows and a piece of classes.  grid: x = tiles, those of one block of rows together
-template <typename T, typename S> __global__ __launch_bounds__(S::kThreads) void head_piece(PieceArgs a)
+// eight neighbouring values as parts, kept where `keep` has ones
+template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int64_t part, float (&v)[8], uint32_t keep)
 {
-    using Product = TileProduct<T, S, kAlongK, kAlongK>;
-    __shared__ __align__(16) char lds[Product::kLds];
-    const int ctiles = (a.classes + S::BN - 1) / S::BN;
-    const int n0 = (blockIdx.x % ctiles) * S::BN, m0 = (blockIdx.x / ctiles) * S::BM;
-    const int F = a.head.F;
-    f32x4 acc[S::FN][S::FM];
 #pragma unroll
-    for (int i = 0; i < S::FN; i++) {
-        const f32x4 b = bias4<T>(a.head.bias, a.c0 + n0 + n_of<S>(i), a.head.C);
+    for (int s = 0; s < PARTS; s++) {
+        u32x4 w;
 #pragma unroll
-        for (int j = 0; j < S::FM; j++) acc[i][j] = b;
-    }
-    const Operand<T> p{static_cast<const T *>(a.head.w) + (int64_t)(a.c0 + n0) * F, F, a.classes - n0};
-    const Operand<T> q{static_cast<const T *>(a.head.x) + (a.row0 + m0) * F, F, a.rows - m0};
-    Product::run(acc, p, q, 0, F, lds);
-    const float all = a.per_row ? 0.f : a.grad[0] / (a.count ? (float)a.count[0] : 1.f);
-#pragma unroll
-    for (int j = 0; j < S::FM; j++) {
-        const int m = m0 + m_of<S>(j);
-        if (m >= a.rows) continue;
-        const int64_t row = a.row0 + m;
-        const int64_t label = head_label(a.head, row);
-        const float g = a.per_row ? a.grad[row] : all, l = a.lse[row];
-#pragma unroll
-        for (int i = 0; i < S::FN; i++) {
-            const int n = n0 + n_of<S>(i);
-            if (n >= a.classes) continue;
-            f32x4 d;
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                d[r] = label < 0 ? 0.f : g * (__expf(acc[i][j][r] - l) - (a.c0 + n + r == label ? 1.f : 0.f));
-            store4<T>(static_cast<T *>(a.d) + m * a.ld + n, d, a.classes - n, true);
+        for (int i = 0; i < 4; i++) {
+            w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+            if (s + 1 < PARTS) {
+                v[2 * i] -= bf16_lo(w[i]);
+                v[2 * i + 1] -= bf16_hi(w[i]);
+            }
+            w[i] &= keep;
         }
+        *reinterpret_cast<u32x4 *>(out + s * part) = w;
     }
+}
+
+// d for a block of rows and a piece of classes.  Classes between the last and ld are written as zero.
+// grid: x = workgroups, each with every gridDim.x-th tile
+template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) void head_piece(PieceArgs a)
+{
+    using Product = StreamProduct<S, kAlongK, kAlongK>;
+    extern __shared__ __align__(16) char lds[];
+    const int ntiles = (a.classes + S::BN - 1) / S::BN, mtiles = (a.rows + S::BM - 1) / S::BM;
+    const HeadArgs &h = a.head;
+    const float all = a.per_row ? 0.f : a.grad[0] / (a.count ? (float)a.count[0] : 1.f);
+    auto corner = [&](int t, int *m0, int *n0) {
+        int m, n;
+        bool exists;
+        tile_at(t, mtiles, ntiles, &m, &n, &exists);
+        *m0 = m * S::BM;
+        *n0 = n * S::BN;
+    };
+    Product::template run<kNoSums>(
+        tiles_of(mtiles, ntiles), lds,
+        [&](int t) {
+            int m0, n0;
+            corner(t, &m0, &n0);
+            return StreamTile{h.w + (int64_t)(a.c0 + n0) * h.ld, h.x + (a.row0 + m0) * h.ld, h.part_w, h.part_x,
+                              h.ld, h.ld, a.classes - n0, a.rows - m0, h.F};
+        },
+        [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *) {
+            int m0, n0;
+            corner(t, &m0, &n0);
+            if (h.bias) {
+#pragma unroll
+                for (int i = 0; i < S::FN; i++) {
+                    const f32x4 b = bias4<T>(h.bias, a.c0 + n0 + Product::n_of(i), h.C);
+#pragma unroll
+                    for (int j = 0; j < S::FM; j++) acc[i][j] += b;
+                }
+            }
+            constexpr float kLog2e = 1.44269504088896341f;
+            const bool edge = n0 + S::BN > a.classes;
+#pragma unroll
+            for (int j = 0; j < S::FM; j++) {
+                const int m = m0 + Product::m_of(j);
+                if (m >= a.rows) continue;
+                const int64_t row = a.row0 + m;
+                const int64_t label = head_label(h, row);
+                const float g = a.per_row ? a.grad[row] : all, l = a.lse[row];
+                const uint32_t keep = label < 0 ? 0u : 0xffffffffu;
+                const int at = label < 0 ? -1 : (int)(label - a.c0 - n0);
+                bf16 *out = a.d + m * (int64_t)a.ld + n0;
+#pragma unroll
+                for (int i = 0; i < S::FN; i += 2) {
+                    const int n = Product::n_of(i);
+                    float d[8];
+                    // z - l is taken before the scaling: both may be large
+#pragma unroll
+                    for (int r = 0; r < 8; r++)
+                        d[r] = g * __builtin_amdgcn_exp2f((acc[i + r / 4][j][r % 4] - l) * kLog2e);
+                    if (at >= n && at < n + 8) {
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+                            if (n + r == at) d[r] -= g;
+                    }
+                    if (edge) {
+                        if (n0 + n >= a.ld) continue;
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+                            if (n0 + n + r >= a.classes) d[r] = 0.f;
+                    }
+                    store_parts8<S::kParts>(out + n, a.part, d, keep);
+                }
+            }
+        });
 }
 
 // out[m][n] = (first ? 0 : acc[m][n]) + sum_k P[n][k] Q[m][k], to `out` when `last`, else to `acc`; with
 // several splits of k every split leaves its sum in part and head_join finishes.
 struct SumArgs {
-    const void *p, *q;
-    int64_t ldp, ldq;
+    const bf16 *p, *q;
+    int64_t part_p, part_q;
+    int ldp, ldq;
     int N, M, K, splits, k_split;
     void *out;          // [M][N]
     float *acc, *part;  // [M][N], [splits][M][N]
@@ -298,45 +439,53 @@ template <typename T> __device__ __forceinline__ void finish4(const SumArgs &a, 
     else store4<float>(acc + at, v, n, a.whole);
 }
 
-// grid: x = tiles x splits, the tiles of one split together
-template <typename T, typename S, Layout PL, Layout QL> __global__ __launch_bounds__(S::kThreads) void head_sum(SumArgs a)
+// grid: x = workgroups, each with every gridDim.x-th tile of a split after the other
+template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_bounds__(S::kThreads, 2) void head_sum(SumArgs a)
 {
-    using Product = TileProduct<T, S, PL, QL>;
-    __shared__ __align__(16) char lds[Product::kLds];
+    using Product = StreamProduct<S, kAcrossK, QL>;
+    extern __shared__ __align__(16) char lds[];
     const int ntiles = (a.N + S::BN - 1) / S::BN, mtiles = (a.M + S::BM - 1) / S::BM;
-    const int tile = blockIdx.x % (ntiles * mtiles), split = blockIdx.x / (ntiles * mtiles);
-    const int n0 = (tile % ntiles) * S::BN, m0 = (tile / ntiles) * S::BM;
-    f32x4 acc[S::FN][S::FM], sums[S::FM];
+    // the splits of a tile are tiles of their own, `mtiles` apart
+    auto corner = [&](int t, int *m0, int *n0, int *split) {
+        int m, n;
+        bool exists;
+        tile_at(t, mtiles * a.splits, ntiles, &m, &n, &exists);
+        *split = m / mtiles;
+        *m0 = (m % mtiles) * S::BM;
+        *n0 = n * S::BN;
+    };
+    Product::template run<SUMS>(
+        tiles_of(mtiles * a.splits, ntiles), lds,
+        [&](int t) {
+            int m0, n0, split;
+            corner(t, &m0, &n0, &split);
+            const int k0 = split * a.k_split, K = max(0, min(a.K - k0, a.k_split));
+            return StreamTile{a.p + (int64_t)k0 * a.ldp + n0,
+                              QL == kAlongK ? a.q + (int64_t)m0 * a.ldq + k0 : a.q + (int64_t)k0 * a.ldq + m0,
+                              a.part_p, a.part_q, a.ldp, a.ldq, a.ldp - n0,
+                              QL == kAlongK ? a.M - m0 : a.ldq - m0, K};
+        },
+        [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *sums) {
+            int m0, n0, split;
+            corner(t, &m0, &n0, &split);
 #pragma unroll
-    for (int j = 0; j < S::FM; j++) {
-        sums[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < S::FM; j++) {
+                const int m = m0 + Product::m_of(j);
+                if (m >= a.M) continue;
+                if (SUMS == kSumQ && n0 == 0 && Product::n_of(0) == 0) {
+                    if (a.splits > 1) a.part_b[(int64_t)split * a.M + m] = sums[j][0];
+                    else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1);
+                }
 #pragma unroll
-        for (int i = 0; i < S::FN; i++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    const T *pb = static_cast<const T *>(a.p), *qb = static_cast<const T *>(a.q);
-    const Operand<T> p{PL == kAlongK ? pb + n0 * a.ldp : pb + n0, a.ldp, a.N - n0};
-    const Operand<T> q{QL == kAlongK ? qb + m0 * a.ldq : qb + m0, a.ldq, a.M - m0};
-    const int k0 = split * a.k_split, k1 = min(a.K, k0 + a.k_split);
-    const bool with_sums = a.out_b && n0 == 0;
-    if (with_sums) Product::template run<kSumQ>(acc, p, q, k0, k1, lds, sums);
-    else Product::run(acc, p, q, k0, k1, lds);
-#pragma unroll
-    for (int j = 0; j < S::FM; j++) {
-        const int m = m0 + m_of<S>(j);
-        if (m >= a.M) continue;
-        if (with_sums && n_of<S>(0) == 0) {
-            if (a.splits > 1) a.part_b[(int64_t)split * a.M + m] = sums[j][0];
-            else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1);
-        }
-#pragma unroll
-        for (int i = 0; i < S::FN; i++) {
-            const int n = n0 + n_of<S>(i);
-            if (n >= a.N) continue;
-            const int64_t at = (int64_t)m * a.N + n;
-            if (a.splits > 1) store4<float>(a.part + (int64_t)split * a.M * a.N + at, acc[i][j], a.N - n, a.whole);
-            else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n);
-        }
-    }
+                for (int i = 0; i < S::FN; i++) {
+                    const int n = n0 + Product::n_of(i);
+                    if (n >= a.N) continue;
+                    const int64_t at = (int64_t)m * a.N + n;
+                    if (a.splits > 1) store4<float>(a.part + (int64_t)split * a.M * a.N + at, acc[i][j], a.N - n, a.whole);
+                    else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n);
+                }
+            }
+        });
 }
 
 // grid: x = results / 1024 (of [M][N], then of [M])
@@ -358,60 +507,101 @@ template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a
     }
 }
 
-template <typename T> using HeadShape = Shape<T, 128, 128, 2, 2>;
-constexpr int kHeadTile = 128;
 
-// ranges of class tiles: enough workgroups for the chip, several tiles each where there are many
-static int head_ranges(int64_t V, int C)
+// workgroups of a launch: as many as are resident at once
+template <typename T> constexpr int head_resident() { return kCus * (int)(160 * 1024 / HeadShape<T>::kLds); }
+template <typename T> static unsigned head_grid(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, head_resident<T>()); }
+
+// ranges of class tiles: as many as fill the chip once
+template <typename T> static int head_ranges(int64_t V, int C)
 {
-    const int64_t tiles = ceil_div(C, kHeadTile), blocks = std::max<int64_t>(1, ceil_div(V, kHeadTile));
-    const int64_t ranges = std::min<int64_t>(tiles, std::max<int64_t>(1, ceil_div(1024, blocks)));
+    using S = HeadShape<T>;
+    const int64_t tiles = ceil_div(C, S::BN), blocks = std::max<int64_t>(1, ceil_div(V, S::BM));
+    const int64_t ranges = std::min<int64_t>(tiles, std::max<int64_t>(1, head_resident<T>() / blocks));
     return (int)ceil_div(tiles, ceil_div(tiles, ranges));
 }
 
-// splits of a sum over K for an [M][N] result: about four workgroups a compute unit, at least 512 steps each
-static int sum_splits(int64_t M, int64_t N, int64_t K)
+// splits of a sum over K for an [M][N] result: the fewest (of at least 512 steps each, up to 32) that
+// leave under an eighth of the workgroups' turns empty, or the best there is
+template <typename T> static int sum_splits(int64_t M, int64_t N, int64_t K)
 {
-    const int64_t tiles = ceil_div(M, kHeadTile) * ceil_div(N, kHeadTile);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(768, tiles), K / 512));
+    using S = HeadShape<T>;
+    const int64_t tiles = ceil_div(M, S::BM) * ceil_div(N, S::BN), resident = head_resident<T>();
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(32, resident / tiles), K / 512));
+    int64_t best = 1;
+    double best_used = 0.0;
+    for (int64_t n = 1; n <= most; n++) {
+        const double used = (double)(tiles * n) / (double)(ceil_div(tiles * n, resident) * resident);
+        if (used > best_used + 0.02) best = n, best_used = used;
+        if (used >= 0.875) break;
+    }
+    return (int)best;
 }
 
 struct Pieces {
     int64_t rows, blocks;      // rows of a block, blocks
     int64_t classes, pieces;   // classes of a piece (whole tiles), pieces
 };
-static Pieces head_pieces(int64_t V, int C)
+template <typename T> static Pieces head_pieces(int64_t V, int C)
 {
+    constexpr int tile = HeadShape<T>::BN;
     Pieces s;
     s.rows = std::min<int64_t>(std::max<int64_t>(V, 1), kBlockRows);
     s.blocks = std::max<int64_t>(1, ceil_div(V, s.rows));
-    s.classes = std::max<int64_t>(kHeadTile, kPieceElements / s.rows / kHeadTile * kHeadTile);
-    s.classes = std::min<int64_t>(s.classes, ceil_div(C, kHeadTile) * kHeadTile);
+    s.classes = std::max<int64_t>(tile, kPieceElements / s.rows / tile * tile);
+    s.classes = std::min<int64_t>(s.classes, ceil_div(C, 8) * 8);
     s.pieces = ceil_div(C, s.classes);
     return s;
 }
 
-// the workspace of the backward pass, in the order it is carved
-struct HeadScratch {
-    size_t d, part, part_b, acc_x, acc_w, acc_b;      // floats (d: bytes)
+// where the parts of x and w come from: the arrays themselves, or copies in the workspace
+template <typename T> static bool parts_in_place(int F) { return sizeof(T) == 2 && F % 8 == 0; }
+static int64_t parts_ld(int F) { return ceil_div(F, 8) * 8; }
+template <typename T> static size_t parts_elements(int64_t R, int F)
+{
+    return parts_in_place<T>(F) ? 0 : (size_t)(R * parts_ld(F) * HeadShape<T>::kParts);
+}
+
+template <typename T> struct HeadScratch {      // of the forward pass, then of the backward pass
+    size_t x = 0, w = 0;                                              // bfloat16
+    size_t stats = 0, at_label = 0, blocks = 0;                       // float2, float, double + int
+    size_t d = 0;                                                     // bfloat16
+    size_t part = 0, part_b = 0, acc_x = 0, acc_w = 0, acc_b = 0;     // float
+    HeadScratch(int64_t V, int F, int C, bool backward)
+    {
+        x = parts_elements<T>(V, F);
+        w = parts_elements<T>(C, F);
+        if (!backward) {
+            stats = (size_t)head_ranges<T>(V, C) * V;
+            at_label = (size_t)V;
+            blocks = (size_t)ceil_div(V, kJoinThreads / kWave);
+            return;
+        }
+        const Pieces s = head_pieces<T>(V, C);
+        d = (size_t)(s.rows * (s.classes + kPad) * HeadShape<T>::kParts);
+        const int64_t sx = sum_splits<T>(s.rows, F, s.classes), sw = sum_splits<T>(s.classes, F, s.rows);
+        part = (size_t)std::max(sx > 1 ? sx * s.rows * F : 0, sw > 1 ? sw * s.classes * F : 0);
+        part_b = (size_t)(sw > 1 ? sw * s.classes : 0);
+        acc_x = s.pieces > 1 ? (size_t)s.rows * F : 0;
+        acc_w = s.blocks > 1 ? (size_t)C * F : 0;
+        acc_b = s.blocks > 1 ? (size_t)C : 0;
+    }
     size_t bytes() const
     {
-        return carve_bytes(d, 1) + carve_bytes(part, 4) + carve_bytes(part_b, 4) + carve_bytes(acc_x, 4) +
-               carve_bytes(acc_w, 4) + carve_bytes(acc_b, 4);
+        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
+               carve_bytes(blocks, 8) + carve_bytes(blocks, 4) + carve_bytes(d, 2) + carve_bytes(part, 4) +
+               carve_bytes(part_b, 4) + carve_bytes(acc_x, 4) + carve_bytes(acc_w, 4) + carve_bytes(acc_b, 4);
     }
 };
-static HeadScratch head_scratch(int64_t V, int F, int C, int32_t dtype)
+
+// more than 64 KB of LDS: the attribute belongs to the function and is set once per instantiation,
+// whichever thread gets here first
+template <auto Kernel> static void raise_lds(size_t bytes)
 {
-    const Pieces s = head_pieces(V, C);
-    HeadScratch n{};
-    n.d = (size_t)(s.rows * s.classes) * (dtype == JGAMD_F32 ? 4 : 2);
-    const int64_t sx = sum_splits(s.rows, F, s.classes), sw = sum_splits(s.classes, F, s.rows);
-    n.part = (size_t)std::max(sx > 1 ? sx * s.rows * F : 0, sw > 1 ? sw * s.classes * F : 0);
-    n.part_b = (size_t)(sw > 1 ? sw * s.classes : 0);
-    n.acc_x = s.pieces > 1 ? (size_t)s.rows * F : 0;
-    n.acc_w = s.blocks > 1 ? (size_t)C * F : 0;
-    n.acc_b = s.blocks > 1 ? (size_t)C : 0;
-    return n;
+    static std::once_flag raised;
+    std::call_once(raised, [&] {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    });
 }
 
 static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int32_t dtype, int32_t reduction)
@@ -424,17 +614,37 @@ static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int3
     if (reduction < 0 || reduction > JGAMD_LOSS_SUM) return fail(JGAMD_ERR_SIZE, "%s: unknown reduction %d", who, reduction);
     return 0;
 }
-static bool head_off_element(int32_t dtype, const void *a, const void *b, const void *c)
+// x and w as parts: copies into the workspace, or the arrays themselves
+template <typename T>
+static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs, bf16 *ws, hipStream_t s)
 {
-    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & (dtype == JGAMD_F32 ? 3 : 1)) != 0;
+    h->ld = (int)parts_ld(h->F);
+    h->part_x = h->V * h->ld;
+    h->part_w = (int64_t)h->C * h->ld;
+    if (parts_in_place<T>(h->F)) {
+        h->x = static_cast<const bf16 *>(x);
+        h->w = static_cast<const bf16 *>(w);
+        return 0;
+    }
+    h->x = xs;
+    h->w = ws;
+    auto copy = [&](const void *src, int64_t R, bf16 *dst, int64_t part) {
+        const int64_t pieces = R * (h->ld / 8);
+        if (pieces > 0)
+            hipLaunchKernelGGL((head_parts<T>), dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, s,
+                               static_cast<const T *>(src), R, h->F, h->ld, dst, part);
+    };
+    copy(x, h->V, xs, h->part_x);
+    copy(w, h->C, ws, h->part_w);
+    return launch_status("linear_cross_entropy");
 }
 
-template <typename T, Layout PL, Layout QL> static int32_t launch_sum(SumArgs a, hipStream_t s)
+template <typename T, Layout QL, Sums SUMS> static int32_t launch_sum(const SumArgs &a, hipStream_t s)
 {
     using S = HeadShape<T>;
-    const int64_t blocks = ceil_div(a.N, S::BN) * ceil_div(a.M, S::BM) * a.splits;
-    if (blocks > 0x7fffffffLL) return fail(JGAMD_ERR_SIZE, "linear_cross_entropy: F=%d is too large", a.N);
-    hipLaunchKernelGGL((head_sum<T, S, PL, QL>), dim3((unsigned)blocks), dim3(S::kThreads), 0, s, a);
+    raise_lds<&head_sum<T, S, QL, SUMS>>(S::kLds);
+    const unsigned grid = head_grid<T>(ceil_div(a.N, S::BN) * ceil_div(a.M, S::BM) * a.splits);
+    hipLaunchKernelGGL((head_sum<T, S, QL, SUMS>), dim3(grid), dim3(S::kThreads), S::kLds, s, a);
     if (a.splits > 1) {
         const int64_t all = (int64_t)a.M * a.N + (a.out_b ? a.M : 0);
         hipLaunchKernelGGL((head_join<T>), dim3((unsigned)ceil_div(all, 1024)), dim3(256), 0, s, a);
@@ -443,51 +653,88 @@ template <typename T, Layout PL, Layout QL> static int32_t launch_sum(SumArgs a,
 }
 
 template <typename T>
-static int32_t head_backward(const HeadArgs &h, const float *lse, const int32_t *count, const float *grad, int32_t reduction,
-                             T *dx, T *dw, T *db, void *ws, int32_t dtype, hipStream_t st)
+static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t reduction, float *loss, int32_t *count,
+                            float *lse, void *ws, hipStream_t st)
 {
     using S = HeadShape<T>;
-    const Pieces s = head_pieces(h.V, h.C);
-    const HeadScratch n = head_scratch(h.V, h.F, h.C, dtype);
+    const HeadScratch<T> n(h.V, h.F, h.C, false);
     Carver carve(ws);
-    T *d = reinterpret_cast<T *>(carve.take<char>(n.d));
+    bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w);
+    float2 *stats = carve.take<float2>(n.stats);
+    float *at_label = carve.take<float>(n.at_label);
+    double *block_sum = carve.take<double>(n.blocks);
+    int32_t *block_count = carve.take<int32_t>(n.blocks);
+    const int mean = reduction == JGAMD_LOSS_MEAN ? 1 : 0;
+    int blocks = 0;
+    if (h.V > 0) {
+        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
+        const int ranges = head_ranges<T>(h.V, h.C);
+        const int per_range = (int)ceil_div(ceil_div(h.C, S::BN), ranges);
+        raise_lds<&head_stats<T, S>>(S::kLds);
+        hipLaunchKernelGGL((head_stats<T, S>), dim3((unsigned)(ceil_div(h.V, S::BM) * ranges)), dim3(S::kThreads), S::kLds,
+                           st, h, ranges, per_range, stats, at_label);
+        int lanes = 1;      // four ranges a lane
+        while (lanes < kWave && lanes * 4 < ranges) lanes *= 2;
+        blocks = (int)ceil_div(h.V, kJoinThreads / lanes);
+        hipLaunchKernelGGL(head_rows, dim3((unsigned)blocks), dim3(kJoinThreads), 0, st, h, ranges, lanes, mean, stats,
+                           at_label, lse, reduction == JGAMD_LOSS_NONE ? loss : nullptr, block_sum, block_count, loss, count);
+    }
+    if (reduction != JGAMD_LOSS_NONE && blocks != 1)
+        hipLaunchKernelGGL(head_total, dim3(1), dim3(kJoinThreads), 0, st, block_sum, block_count, blocks, mean, loss, count);
+    return launch_status("linear_cross_entropy_fwd");
+}
+
+template <typename T>
+static int32_t head_backward(HeadArgs h, const void *x, const void *w, const float *lse, const int32_t *count,
+                             const float *grad, int32_t reduction, T *dx, T *dw, T *db, void *ws, hipStream_t st)
+{
+    using S = HeadShape<T>;
+    const Pieces s = head_pieces<T>(h.V, h.C);
+    const HeadScratch<T> n(h.V, h.F, h.C, true);
+    Carver carve(ws);
+    bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w), *d = carve.take<bf16>(n.d);
     float *part = carve.take<float>(n.part), *part_b = carve.take<float>(n.part_b);
     float *acc_x = carve.take<float>(n.acc_x), *acc_w = carve.take<float>(n.acc_w), *acc_b = carve.take<float>(n.acc_b);
+    if (h.V > 0)
+        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
+    if (h.V == 0) h.ld = (int)parts_ld(h.F);
+    const int ldd = (int)s.classes + kPad;
+    const int64_t part_d = s.rows * ldd;
     auto whole = [](int N, const void *p) { return N % 4 == 0 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0; };
     for (int64_t b = 0; b < s.blocks; b++) {
         const int64_t row0 = b * s.rows;
         const int rows = (int)std::min<int64_t>(s.rows, h.V - row0);
-        const T *x = static_cast<const T *>(h.x) + row0 * h.F;
         for (int64_t c = 0; c < s.pieces; c++) {
             const int c0 = (int)(c * s.classes), classes = (int)std::min<int64_t>(s.classes, h.C - c0);
             if (rows > 0) {
                 const PieceArgs a{h, lse, grad, reduction == JGAMD_LOSS_MEAN ? count : nullptr,
-                                  reduction == JGAMD_LOSS_NONE, row0, rows, c0, classes, d, s.classes};
-                const int64_t blocks = ceil_div(classes, S::BN) * ceil_div(rows, S::BM);
-                hipLaunchKernelGGL((head_piece<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, a);
+                                  reduction == JGAMD_LOSS_NONE, row0, rows, c0, classes, d, part_d, ldd};
+                raise_lds<&head_piece<T, S>>(S::kLds);
+                hipLaunchKernelGGL((head_piece<T, S>), dim3(head_grid<T>(ceil_div(classes, S::BN) * ceil_div(rows, S::BM))),
+                                   dim3(S::kThreads), S::kLds, st, a);
                 if (int32_t rc = launch_status("linear_cross_entropy_bwd")) return rc;
             }
-            const T *w = static_cast<const T *>(h.w) + (int64_t)c0 * h.F;
+            SumArgs a{};
+            a.q = d, a.part_q = part_d, a.ldq = ldd, a.ldp = h.ld, a.N = h.F, a.part = part;
             if (dx && rows > 0) {
-                SumArgs a{};
-                a.p = w, a.ldp = h.F, a.q = d, a.ldq = s.classes;
-                a.N = h.F, a.M = rows, a.K = classes;
-                a.splits = sum_splits(s.rows, h.F, s.classes);
+                a.p = h.w + (int64_t)c0 * h.ld, a.part_p = h.part_w;
+                a.M = rows, a.K = classes;
+                a.splits = sum_splits<T>(s.rows, h.F, s.classes);
                 a.k_split = (int)(ceil_div(ceil_div(s.classes, a.splits), 64) * 64);
-                a.out = dx + row0 * h.F, a.acc = acc_x, a.part = part;
+                a.out = dx + row0 * h.F, a.acc = acc_x;
                 a.first = c == 0, a.last = c == s.pieces - 1, a.whole = whole(h.F, a.out);
-                if (int32_t rc = launch_sum<T, kAcrossK, kAlongK>(a, st)) return rc;
+                if (int32_t rc = launch_sum<T, kAlongK, kNoSums>(a, st)) return rc;
             }
-            if (dw || db) {
-                SumArgs a{};
-                a.p = x, a.ldp = h.F, a.q = d, a.ldq = s.classes;
-                a.N = h.F, a.M = classes, a.K = rows;
-                a.splits = sum_splits(s.classes, h.F, s.rows);
+            if (dw) {
+                a.p = h.x + row0 * h.ld, a.part_p = h.part_x;
+                a.M = classes, a.K = rows;
+                a.splits = sum_splits<T>(s.classes, h.F, s.rows);
                 a.k_split = (int)(ceil_div(ceil_div(s.rows, a.splits), 64) * 64);
-                a.out = dw + (int64_t)c0 * h.F, a.acc = acc_w + (s.blocks > 1 ? (int64_t)c0 * h.F : 0), a.part = part;
-                a.out_b = db ? db + c0 : nullptr, a.acc_b = acc_b + (s.blocks > 1 ? c0 : 0), a.part_b = part_b;
+                a.out = dw + (int64_t)c0 * h.F, a.acc = s.blocks > 1 ? acc_w + (int64_t)c0 * h.F : nullptr;
+                a.out_b = db ? db + c0 : nullptr, a.acc_b = s.blocks > 1 ? acc_b + c0 : nullptr, a.part_b = part_b;
                 a.first = b == 0, a.last = b == s.blocks - 1, a.whole = whole(h.F, a.out);
-                if (int32_t rc = launch_sum<T, kAcrossK, kAcrossK>(a, st)) return rc;
+                const int32_t rc = db ? launch_sum<T, kAcrossK, kSumQ>(a, st) : launch_sum<T, kAcrossK, kNoSums>(a, st);
+                if (rc) return rc;
             }
         }
     }
@@ -499,11 +746,34 @@ static int32_t head_backward(const HeadArgs &h, const float *lse, const int32_t 
 using namespace jg;
 #define JG_EXPORT extern "C" __attribute__((visibility("default")))
 
-static size_t head_fwd_bytes(int64_t V, int32_t C)
+static size_t head_bytes(int64_t V, int32_t F, int32_t C, int32_t dtype, bool backward)
 {
-    const size_t blocks = (size_t)ceil_div(V, kJoinThreads);
-    return carve_bytes((size_t)head_ranges(V, C) * V, 8) + carve_bytes((size_t)V, 4) + carve_bytes(blocks, 8) +
-           carve_bytes(blocks, 4);
+    return dtype == JGAMD_F32 ? HeadScratch<float>(V, F, C, backward).bytes() : HeadScratch<bf16>(V, F, C, backward).bytes();
+}
+
+// what the two entry points ask of their arrays
+static int32_t head_arrays(const char *who, int32_t dtype, const void *x, const void *w, const void *bias, const void *labels,
+                           int32_t i64, int32_t F, const void *ws, size_t ws_bytes, size_t need)
+{
+    const uintptr_t element = dtype == JGAMD_F32 ? 3 : F % 8 == 0 ? 15 : 1;
+    if ((((uintptr_t)x | (uintptr_t)w) & element) != 0)
+        return fail(JGAMD_ERR_ALIGN, "%s: x / w not aligned to %d bytes", who, (int)element + 1);
+    if (((uintptr_t)bias & (dtype == JGAMD_F32 ? 3 : 1)) != 0 || ((uintptr_t)labels & (i64 ? 7 : 3)) != 0)
+        return fail(JGAMD_ERR_ALIGN, "%s: bias / labels do not start at a multiple of their element's size", who);
+    if (need > 0 && (!ws || ws_bytes < need))
+        return fail(JGAMD_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", who, ws ? ws_bytes : (size_t)0, need);
+    if (need > 0 && ((uintptr_t)ws & 255) != 0) return fail(JGAMD_ERR_ALIGN, "%s: workspace not 256-byte aligned", who);
+    return 0;
+}
+
+static HeadArgs head_args(const void *bias, const void *labels, int32_t i64, int64_t V, int32_t F, int32_t C)
+{
+    HeadArgs h{};
+    h.bias = bias;
+    h.y32 = i64 ? nullptr : static_cast<const int32_t *>(labels);
+    h.y64 = i64 ? static_cast<const int64_t *>(labels) : nullptr;
+    h.V = V, h.F = F, h.C = C;
+    return h;
 }
 
 JG_EXPORT int32_t jgamd_linear_cross_entropy_workspace(int64_t V, int32_t F, int32_t C, int32_t dtype, int32_t backward,
@@ -511,7 +781,7 @@ JG_EXPORT int32_t jgamd_linear_cross_entropy_workspace(int64_t V, int32_t F, int
 {
     if (!bytes) return fail(JGAMD_ERR_NULL, "linear_cross_entropy_workspace: bytes is NULL");
     if (int32_t rc = head_check("linear_cross_entropy_workspace", V, F, C, dtype, 0)) return rc;
-    *bytes = backward ? head_scratch(V, F, C, dtype).bytes() : head_fwd_bytes(V, C);
+    *bytes = head_bytes(V, F, C, dtype, backward != 0);
     return 0;
 }
 
@@ -520,44 +790,18 @@ JG_EXPORT int32_t jgamd_linear_cross_entropy_fwd(const void *x, const void *w, c
                                                  int32_t reduction, float *loss, int32_t *count, float *lse, void *ws,
                                                  size_t ws_bytes, void *stream)
 {
-    if (int32_t rc = head_check("linear_cross_entropy_fwd", V, F, C, dtype, reduction)) return rc;
-    if (!count || (reduction != JGAMD_LOSS_NONE && !loss))
-        return fail(JGAMD_ERR_NULL, "linear_cross_entropy_fwd: loss / count is NULL");
-    if (V > 0 && (!x || !w || !labels || !lse || !loss)) return fail(JGAMD_ERR_NULL, "linear_cross_entropy_fwd: NULL array");
-    if (head_off_element(dtype, x, w, bias) || ((uintptr_t)labels & (labels_are_i64 ? 7 : 3)) != 0 ||
-        (((uintptr_t)loss | (uintptr_t)count | (uintptr_t)lse) & 3) != 0)
-        return fail(JGAMD_ERR_ALIGN, "linear_cross_entropy_fwd: an array does not start at a multiple of its element's size");
-    const size_t need = head_fwd_bytes(V, C);
-    if (need > 0 && (!ws || ws_bytes < need))
-        return fail(JGAMD_ERR_WORKSPACE, "linear_cross_entropy_fwd: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, need);
-    if (need > 0 && ((uintptr_t)ws & 255) != 0)
-        return fail(JGAMD_ERR_ALIGN, "linear_cross_entropy_fwd: workspace not 256-byte aligned");
+    const char *who = "linear_cross_entropy_fwd";
+    if (int32_t rc = head_check(who, V, F, C, dtype, reduction)) return rc;
+    if (reduction != JGAMD_LOSS_NONE && (!loss || !count)) return fail(JGAMD_ERR_NULL, "%s: loss / count is NULL", who);
+    if (V > 0 && (!x || !w || !labels || !lse || !loss)) return fail(JGAMD_ERR_NULL, "%s: NULL array", who);
+    if ((((uintptr_t)loss | (uintptr_t)count | (uintptr_t)lse) & 3) != 0)
+        return fail(JGAMD_ERR_ALIGN, "%s: loss / count / lse not 4-byte aligned", who);
+    const size_t need = head_bytes(V, F, C, dtype, false);
+    if (int32_t rc = head_arrays(who, dtype, x, w, bias, labels, labels_are_i64, F, ws, ws_bytes, need)) return rc;
+    const HeadArgs h = head_args(bias, labels, labels_are_i64, V, F, C);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int ranges = head_ranges(V, C), blocks = (int)ceil_div(V, kJoinThreads);
-    const int per_range = (int)ceil_div(ceil_div(C, kHeadTile), ranges);
-    Carver carve(ws);
-    float2 *stats = carve.take<float2>((size_t)ranges * V);
-    float *at_label = carve.take<float>((size_t)V);
-    double *block_sum = carve.take<double>((size_t)blocks);
-    int32_t *block_count = carve.take<int32_t>((size_t)blocks);
-    const HeadArgs a{x, w, bias, labels_are_i64 ? nullptr : static_cast<const int32_t *>(labels),
-                     labels_are_i64 ? static_cast<const int64_t *>(labels) : nullptr, V, F, C};
-    if (V > 0) {
-        const int64_t grid = ceil_div(V, kHeadTile) * ranges;
-        if (grid > 0x7fffffffLL) return fail(JGAMD_ERR_SIZE, "linear_cross_entropy_fwd: V=%lld is too large", (long long)V);
-        if (dtype == JGAMD_F32)
-            hipLaunchKernelGGL((head_stats<float, HeadShape<float>>), dim3((unsigned)grid), dim3(HeadShape<float>::kThreads),
-                               0, st, a, ranges, per_range, stats, at_label);
-        else
-            hipLaunchKernelGGL((head_stats<bf16, HeadShape<bf16>>), dim3((unsigned)grid), dim3(HeadShape<bf16>::kThreads), 0,
-                               st, a, ranges, per_range, stats, at_label);
-        hipLaunchKernelGGL(head_rows, dim3((unsigned)blocks), dim3(kJoinThreads), 0, st, a, ranges, stats, at_label, lse,
-                           reduction == JGAMD_LOSS_NONE ? loss : nullptr, block_sum, block_count);
-    }
-    if (reduction != JGAMD_LOSS_NONE)
-        hipLaunchKernelGGL(head_total, dim3(1), dim3(kJoinThreads), 0, st, block_sum, block_count, blocks,
-                           reduction == JGAMD_LOSS_MEAN ? 1 : 0, loss, count);
-    return launch_status("linear_cross_entropy_fwd");
+    return dtype == JGAMD_F32 ? head_forward<float>(h, x, w, reduction, loss, count, lse, ws, st)
+                              : head_forward<bf16>(h, x, w, reduction, loss, count, lse, ws, st);
 }
 
 JG_EXPORT int32_t jgamd_linear_cross_entropy_bwd(const void *x, const void *w, const void *bias, const void *labels,
@@ -566,24 +810,22 @@ JG_EXPORT int32_t jgamd_linear_cross_entropy_bwd(const void *x, const void *w, c
                                                  int32_t reduction, void *dx, void *dw, void *db, void *ws,
                                                  size_t ws_bytes, void *stream)
 {
-    if (int32_t rc = head_check("linear_cross_entropy_bwd", V, F, C, dtype, reduction)) return rc;
-    if (db && !dw) return fail(JGAMD_ERR_NULL, "linear_cross_entropy_bwd: db without dw");
+    const char *who = "linear_cross_entropy_bwd";
+    if (int32_t rc = head_check(who, V, F, C, dtype, reduction)) return rc;
+    if (db && !dw) return fail(JGAMD_ERR_NULL, "%s: db without dw", who);
     if (V > 0 && (!x || !w || !labels || !lse || !grad || (reduction == JGAMD_LOSS_MEAN && !count)))
-        return fail(JGAMD_ERR_NULL, "linear_cross_entropy_bwd: NULL array");
-    if (head_off_element(dtype, x, w, bias) || head_off_element(dtype, dx, dw, db) ||
-        ((uintptr_t)labels & (labels_are_i64 ? 7 : 3)) != 0 || (((uintptr_t)lse | (uintptr_t)count | (uintptr_t)grad) & 3) != 0)
-        return fail(JGAMD_ERR_ALIGN, "linear_cross_entropy_bwd: an array does not start at a multiple of its element's size");
+        return fail(JGAMD_ERR_NULL, "%s: NULL array", who);
+    const uintptr_t outs = (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)db;
+    if ((outs & (dtype == JGAMD_F32 ? 3 : 1)) != 0 || (((uintptr_t)lse | (uintptr_t)count | (uintptr_t)grad) & 3) != 0)
+        return fail(JGAMD_ERR_ALIGN, "%s: an array does not start at a multiple of its element's size", who);
     if (!dx && !dw) return 0;
-    const size_t need = head_scratch(V, F, C, dtype).bytes();
-    if (!ws || ws_bytes < need)
-        return fail(JGAMD_ERR_WORKSPACE, "linear_cross_entropy_bwd: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, need);
-    if (((uintptr_t)ws & 255) != 0) return fail(JGAMD_ERR_ALIGN, "linear_cross_entropy_bwd: workspace not 256-byte aligned");
-    const HeadArgs h{x, w, bias, labels_are_i64 ? nullptr : static_cast<const int32_t *>(labels),
-                     labels_are_i64 ? static_cast<const int64_t *>(labels) : nullptr, V, F, C};
+    const size_t need = head_bytes(V, F, C, dtype, true);
+    if (int32_t rc = head_arrays(who, dtype, x, w, bias, labels, labels_are_i64, F, ws, ws_bytes, need)) return rc;
+    const HeadArgs h = head_args(bias, labels, labels_are_i64, V, F, C);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == JGAMD_F32)
-        return head_backward<float>(h, lse, count, grad, reduction, static_cast<float *>(dx), static_cast<float *>(dw),
-                                    static_cast<float *>(db), ws, dtype, st);
-    return head_backward<bf16>(h, lse, count, grad, reduction, static_cast<bf16 *>(dx), static_cast<bf16 *>(dw),
-                               static_cast<bf16 *>(db), ws, dtype, st);
+        return head_backward<float>(h, x, w, lse, count, grad, reduction, static_cast<float *>(dx), static_cast<float *>(dw),
+                                    static_cast<float *>(db), ws, st);
+    return head_backward<bf16>(h, x, w, lse, count, grad, reduction, static_cast<bf16 *>(dx), static_cast<bf16 *>(dw),
+                               static_cast<bf16 *>(db), ws, st);
 }

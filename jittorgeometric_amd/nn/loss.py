@@ -147,5 +147,6 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.dtype != x.dtype:
             raise _lib.JgamdError("linear_cross_entropy: %s is %s, x is %s" % (name, t.dtype, x.dtype))
-    return _LinearCrossEntropy.apply(x.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(),
-                                     target.contiguous(), _REDUCTIONS[reduction])
+    x, weight = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (x.contiguous(), weight.contiguous()))
+    return _LinearCrossEntropy.apply(x, weight, None if bias is None else bias.contiguous(), target.contiguous(),
+                                     _REDUCTIONS[reduction])
