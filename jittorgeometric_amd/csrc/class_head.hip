@@ -34,10 +34,10 @@ constexpr int kPad = 128;      // classes between the rows of d: rows a power of
 // float: three parts an operand, 256 x 128 results, two stages (144 KB).
 template <typename T> struct HeadShapeOf;
 template <> struct HeadShapeOf<bf16> {
-    using S = StreamShape<1, 256, 128, 2, 2, 3>;
+    using S = StreamShape<1, 256, 256, 2, 4, 64, 2>;
 };
 template <> struct HeadShapeOf<float> {
-    using S = StreamShape<3, 256, 128, 4, 2, 2>;
+    using S = StreamShape<3, 256, 128, 4, 2, 32, 2>;
 };
 template <typename T> using HeadShape = typename HeadShapeOf<T>::S;
 

@@ -2,7 +2,7 @@
 // addresses: tiles go from memory to LDS directly (buffer_load ... lds), several steps ahead, and a
 // workgroup that owns several tiles keeps loading across their borders.
 //
-// A step is 32 values of k.  STAGES steps have room in LDS; while one is multiplied, the next
+// A step is 32 or 64 values of k.  STAGES steps have room in LDS; while one is multiplied, the next
 // STAGES - 1 are loaded or on their way.  Per step a wavefront waits until its own loads of that step
 // have landed (all but the newest (STAGES - 2) steps' loads) and until its LDS reads of the step
 // before are done, then one barrier makes every wavefront's loads visible and the oldest stage free
@@ -10,7 +10,7 @@
 // descriptor's range, which the hardware answers with zeros: k past the end adds nothing.  Rows past
 // the last of a tile repeat a row that exists and are not stored.
 //
-// The LDS image is that of Place<BR, 32, LAY>: a wavefront's load writes 1 KB in lane order, so the
+// The LDS image is in lines of 32 or 64 k, or of the tile's rows: a wavefront's load writes 1 KB in lane order, so the
 // permutation is applied to the address each lane asks for.
 //
 // Which row of P stands at which row of a 16 x 16 fragment is free.  With P along k the fragments
@@ -24,7 +24,6 @@
 
 namespace jg {
 
-constexpr int kStreamStep = 32;
 constexpr uint32_t kStreamRange = 0x40000000u;      // bytes a lane's offset may span; past it reads zero
 
 // One tile of the product: p[row][k] or p[k][row] as bfloat16 parts `part` elements apart.
@@ -37,16 +36,16 @@ struct StreamTile {
     int K;
 };
 
-template <int PARTS, int BN_, int BM_, int WN_, int WM_, int STAGES_> struct StreamShape {
-    static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, kStages = STAGES_, kParts = PARTS;
+template <int PARTS, int BN_, int BM_, int WN_, int WM_, int STEP_, int STAGES_> struct StreamShape {
+    static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, kStep = STEP_, kStages = STAGES_, kParts = PARTS;
     static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
     static constexpr int FN = BN / WN / 16, FM = BM / WM / 16;
-    static constexpr int kLoadsP = BN / 16 / kWaves, kLoadsQ = BM / 16 / kWaves;      // of a wavefront, step and part
+    static constexpr int kLoadsP = BN * kStep / 512 / kWaves, kLoadsQ = BM * kStep / 512 / kWaves;      // of a wavefront, step and part
     static constexpr int kLoads = (kLoadsP + kLoadsQ) * PARTS;
-    static constexpr int kPartP = BN * kStreamStep * 2, kPartQ = BM * kStreamStep * 2;
+    static constexpr int kPartP = BN * kStep * 2, kPartQ = BM * kStep * 2;
     static constexpr int kStage = (kPartP + kPartQ) * PARTS;
     static constexpr int kLds = kStage * kStages;
-    static_assert(kLoadsP >= 1 && kLoadsQ >= 1 && kLoads * (kStages - 2) < 64, "");
+    static_assert(kLoadsP >= 1 && kLoadsQ >= 1 && kLoads * (kStages - 2) < 64 && (kStep == 32 || kStep == 64), "");
 };
 
 // Four fragments of 16 rows whose LDS lines run along the rows, by transposing reads (tile_product.h's
@@ -103,18 +102,20 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
         return (wave_in_block() % S::WM) * (S::BM / S::WM) + j * 16 + (lane_id() & 15);
     }
 
-    // the turn of a row's 16-byte pieces: the eight rows that are read at a time (0 .. 7 of Q; 0 .. 3
-    // and 8 .. 11 of P in pairs) fall on different banks
+    static constexpr int kRowPieces = S::kStep / 8;      // of 16 bytes, of a row along k
+
+    // The turn of a row's pieces: the eight rows that are read at a time (0 .. 7 of Q; 0 .. 3 and 8 .. 11
+    // of P in pairs) fall on different banks.  Rows of 64 bytes alternate between two halves by themselves.
     template <bool PAIRS> __device__ __forceinline__ static int turn(int row)
     {
-        return PAIRS ? ((row >> 1) & 1) | ((row >> 2) & 2) : (row >> 1) & 3;
+        const int eight = PAIRS ? (row & 3) | ((row >> 1) & 4) : row & 7;
+        return kRowPieces == 8 ? eight : eight >> 1;
     }
-    __device__ __forceinline__ static bf16x8 fragment_p(const char *lds, int row0, int i)
+    // fragment of 16 rows along k at step kk of a stage, this lane's row given
+    template <bool PAIRS> __device__ __forceinline__ static bf16x8 fragment_along(const char *lds, int row, int kk)
     {
-        if (!kPairs) return fragment<S::BN, kStreamStep, PL>(lds, row0 + 16 * i, 0);
-        const int t = lane_id() & 15, g = lane_id() >> 4;
-        const int row = row0 + (i >> 1) * 32 + (t >> 2) * 8 + (i & 1) * 4 + (t & 3);
-        return *reinterpret_cast<const bf16x8 *>(lds + row * 64 + ((g ^ turn<true>(row)) << 4));
+        const int g = lane_id() >> 4;
+        return *reinterpret_cast<const bf16x8 *>(lds + row * (2 * S::kStep) + (((kk / 8 + g) ^ turn<PAIRS>(row)) << 4));
     }
 
     // the addresses that this lane asks for, relative to the tile's (k = k0) corner
@@ -123,7 +124,7 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
         __device__ __forceinline__ static int k_of(int u)
         {
             const int id = (wave_in_block() * LOADS + u) * kWave + lane_id();
-            if (LAY == kAlongK) return ((id & 3) ^ turn<PAIRS>(id >> 2)) * 8;
+            if (LAY == kAlongK) return ((id % kRowPieces) ^ turn<PAIRS>(id / kRowPieces)) * 8;
             return id / (BR / 8);
         }
         __device__ __forceinline__ void place(int ld, int rows)
@@ -132,7 +133,7 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
             for (int u = 0; u < LOADS; u++) {
                 const int id = (wave_in_block() * LOADS + u) * kWave + lane_id();
                 if (LAY == kAlongK) {
-                    off[u] = (uint32_t)min(id >> 2, rows - 1) * (uint32_t)(2 * ld) + 2 * k_of(u);
+                    off[u] = (uint32_t)min(id / kRowPieces, rows - 1) * (uint32_t)(2 * ld) + 2 * k_of(u);
                 } else {
                     const int k = id / (BR / 8), pos = id % (BR / 8);
                     const int by = (k & 3) | ((k >> 1) & 4);
@@ -199,7 +200,7 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
                                  left, stage + S::kParts * S::kPartP + s * S::kPartQ);
             }
             load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
-            load_k += kStreamStep;
+            load_k += S::kStep;
             if (load_k >= in.K && load_tile < tiles) {
                 load_k = 0;
                 if (++load_tile < tiles) {
@@ -217,9 +218,9 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
         const int line_row = 4 * (lane_id() & 3), line_k = 8 * (lane_id() >> 4) + ((lane_id() >> 2) & 3);
         const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char *)lds;
 #pragma unroll
-        for (int i = 0; i < S::FN; i++) across_p[i] = lds_at + Place<S::BN, kStreamStep, kAcrossK>::at(wn + 16 * i + line_row, line_k);
+        for (int i = 0; i < S::FN; i++) across_p[i] = lds_at + Place<S::BN, S::kStep, kAcrossK>::at(wn + 16 * i + line_row, line_k);
 #pragma unroll
-        for (int j = 0; j < S::FM; j++) across_q[j] = lds_at + S::kParts * S::kPartP + Place<S::BM, kStreamStep, kAcrossK>::at(wm + 16 * j + line_row, line_k);
+        for (int j = 0; j < S::FM; j++) across_q[j] = lds_at + S::kParts * S::kPartP + Place<S::BM, S::kStep, kAcrossK>::at(wm + 16 * j + line_row, line_k);
         int stage_at = 0;
         for (int t = 0; t < tiles; t++) {
             f32x4 acc[S::FN][S::FM], sums[kSums];
@@ -239,51 +240,59 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
                 const char *lp = lds + stage, *lq = lp + S::kParts * S::kPartP;
                 stage_at = stage_at + 1 == S::kStages ? 0 : stage_at + 1;
                 bf16x8 fp[S::kParts][S::FN], fq[S::kParts][S::FM];
-                auto read = [&](auto part) {
-                    constexpr int s = decltype(part)::value;
+                auto read = [&](auto part, auto at_k) {
+                    constexpr int s = decltype(part)::value, kk = decltype(at_k)::value;
                     if constexpr (QL == kAlongK) {
 #pragma unroll
                         for (int j = 0; j < S::FM; j++)
-                            fq[s][j] = fragment<S::BM, kStreamStep, QL>(lq + s * S::kPartQ, wm + 16 * j, 0);
+                            fq[s][j] = fragment_along<false>(lq + s * S::kPartQ, wm + 16 * j + (lane_id() & 15), kk);
                     } else {
                         uint32_t at[S::FM];
 #pragma unroll
                         for (int j = 0; j < S::FM; j++) at[j] = across_q[j] + stage;
 #pragma unroll
-                        for (int j = 0; j < S::FM; j += 4) fragments_across<s * S::kPartQ, 8 * S::BM>(at + j, &fq[s][j]);
+                        for (int j = 0; j < S::FM; j += 4)
+                            fragments_across<s * S::kPartQ + kk * 2 * S::BM, 8 * S::BM>(at + j, &fq[s][j]);
                     }
                     if constexpr (PL == kAlongK) {
+                        const int t = lane_id() & 15;
 #pragma unroll
-                        for (int i = 0; i < S::FN; i++) fp[s][i] = fragment_p(lp + s * S::kPartP, wn, i);
+                        for (int i = 0; i < S::FN; i++)
+                            fp[s][i] = fragment_along<true>(
+                                lp + s * S::kPartP, wn + (i >> 1) * 32 + (t >> 2) * 8 + (i & 1) * 4 + (t & 3), kk);
                     } else {
                         uint32_t at[S::FN];
 #pragma unroll
                         for (int i = 0; i < S::FN; i++) at[i] = across_p[i] + stage;
 #pragma unroll
                         for (int i = 0; i < S::FN; i += 4) {
-                            fragments_across<s * S::kPartP, 8 * S::BN>(at + i, &fp[s][i]);
+                            fragments_across<s * S::kPartP + kk * 2 * S::BN, 8 * S::BN>(at + i, &fp[s][i]);
                             if constexpr (S::kParts == 1) multiply<1>(acc, fp, fq, i, i + 4);      // while the next are read
                         }
                     }
                 };
-                read(std::integral_constant<int, 0>());
-                if constexpr (S::kParts == 3) {
-                    read(std::integral_constant<int, 1>());
-                    read(std::integral_constant<int, 2>());
-                }
-                if constexpr (S::kParts > 1 || PL == kAlongK) multiply<S::kParts>(acc, fp, fq, 0, S::FN);
-                if (SUMS != kNoSums) {
-                    const uint32_t one = 0x3f803f80u;      // two bfloat16 ones
-                    const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one, one, one, one});
+                auto step = [&](auto at_k) {
+                    read(std::integral_constant<int, 0>(), at_k);
+                    if constexpr (S::kParts == 3) {
+                        read(std::integral_constant<int, 1>(), at_k);
+                        read(std::integral_constant<int, 2>(), at_k);
+                    }
+                    if constexpr (S::kParts > 1 || PL == kAlongK) multiply<S::kParts>(acc, fp, fq, 0, S::FN);
+                    if (SUMS != kNoSums) {
+                        const uint32_t one = 0x3f803f80u;      // two bfloat16 ones
+                        const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one, one, one, one});
 #pragma unroll
-                    for (int s = S::kParts - 1; s >= 0; s--)
+                        for (int s = S::kParts - 1; s >= 0; s--)
 #pragma unroll
-                        for (int i = 0; i < kSums; i++)
-                            sums[i] = SUMS == kSumP
-                                          ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[s][i], ones, sums[i], 0, 0, 0)
-                                          : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fq[s][i], sums[i], 0, 0, 0);
-                }
-                k += kStreamStep;
+                            for (int i = 0; i < kSums; i++)
+                                sums[i] = SUMS == kSumP
+                                              ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[s][i], ones, sums[i], 0, 0, 0)
+                                              : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fq[s][i], sums[i], 0, 0, 0);
+                    }
+                };
+                step(std::integral_constant<int, 0>());
+                if constexpr (S::kStep == 64) step(std::integral_constant<int, 32>());
+                k += S::kStep;
             } while (k < K);
             done(t, acc, sums);
         }
