@@ -16,8 +16,8 @@
 //
 // Bound by the matrix units from some hundred rows on, by reading w below that.
 #include <algorithm>
-#include <mutex>
 
+#include "lds_size.h"
 #include "stream_product.h"
 
 namespace jg {
@@ -593,16 +593,6 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
                carve_bytes(part_b, 4) + carve_bytes(acc_x, 4) + carve_bytes(acc_w, 4) + carve_bytes(acc_b, 4);
     }
 };
-
-// more than 64 KB of LDS: the attribute belongs to the function and is set once per instantiation,
-// whichever thread gets here first
-template <auto Kernel> static void raise_lds(size_t bytes)
-{
-    static std::once_flag raised;
-    std::call_once(raised, [&] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    });
-}
 
 static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int32_t dtype, int32_t reduction)
 {

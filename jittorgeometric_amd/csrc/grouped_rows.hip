@@ -15,7 +15,8 @@
 // kernel: no atomics, the same bits every time.
 #include <algorithm>
 
-#include "tile_product.h"
+#include "lds_size.h"
+#include "stream_product.h"
 
 namespace jg {
 
@@ -55,16 +56,15 @@ struct Run {
     int slot;      // pieces of earlier types that have more than one
 };
 
-// The `wanted`-th piece of at most `step` rows, counted over the types in order.  With `typed`
-// false the rows before the first and behind the last type are runs of their own; with it true
-// only types count, and a type without rows has one (empty) piece.  Returns false past the last.
-template <int THREADS>
-__device__ __forceinline__ bool find_run(const int32_t *__restrict__ off, int G, int M, int step, int wanted, bool typed,
-                                         Run *run)
+// Pieces of at most `step` rows, counted over the types in order.  Looks up `count` of them: the i-th is
+// number wanted(i); runs[i].pieces is 0 where there is no such piece.  With `typed` false the rows
+// before the first and behind the last type are runs of their own; with it true only types count, and
+// a type without rows has one (empty) piece.  The workgroup calls it; runs[] lies in LDS.
+template <int THREADS, typename Wanted>
+__device__ __forceinline__ void find_runs(const int32_t *__restrict__ off, int G, int M, int step, bool typed, int count,
+                                          Wanted &&wanted, Run *runs)
 {
     __shared__ int wave_totals[THREADS / kWave];
-    __shared__ Run found;
-    __shared__ int hit;
     // thread t reads `per` neighbouring offsets: 0 .. G + 1 with off[G + 1] taken as M
     const int n = G + 2;
     const int per = (n + THREADS - 1) / THREADS;
@@ -84,7 +84,7 @@ __device__ __forceinline__ bool find_run(const int32_t *__restrict__ off, int G,
             const bool counted = !typed || (i >= 1 && i <= G);
             int np = counted && rows > 0 ? (rows - 1) / step + 1 : 0;
             if (typed && counted && np == 0) np = 1;
-            body(i - 1, begin, rows, np);
+            if (np > 0) body(i - 1, begin, rows, np);
             begin = high;
         }
     };
@@ -93,24 +93,35 @@ __device__ __forceinline__ bool find_run(const int32_t *__restrict__ off, int G,
         slots += np > 1 ? np : 0;
     });
     int all, ignored;
-    int at = block_exclusive<THREADS, false>(pieces, wave_totals, &all);
-    int slot = block_exclusive<THREADS, false>(slots, wave_totals, &ignored);
-    if (threadIdx.x == 0) hit = 0;
-    __syncthreads();
-    if (wanted >= at && wanted < at + pieces) {
-        each([&](int type, int begin, int rows, int np) {
-            if (wanted >= at && wanted < at + np) {
-                const int piece = wanted - at;
-                found = Run{type, begin + piece * step, min(step, rows - piece * step), piece, np, slot};
-                hit = 1;
-            }
-            at += np;
-            slot += np > 1 ? np : 0;
-        });
+    const int at0 = block_exclusive<THREADS, false>(pieces, wave_totals, &all);
+    const int slot0 = block_exclusive<THREADS, false>(slots, wave_totals, &ignored);
+    for (int k = 0; k < count; k++) {
+        const int want = wanted(k);
+        if (want >= at0 && want < at0 + pieces) {
+            int at = at0, slot = slot0;
+            each([&](int type, int begin, int rows, int np) {
+                if (want >= at && want < at + np) {
+                    const int piece = want - at;
+                    runs[k] = Run{type, begin + piece * step, min(step, rows - piece * step), piece, np, slot};
+                }
+                at += np;
+                slot += np > 1 ? np : 0;
+            });
+        }
+        if (threadIdx.x == 0 && want >= all) runs[k].pieces = 0;
     }
     __syncthreads();
+}
+
+// one of them, for workgroup blockIdx.x's single tile; false where there is none
+template <int THREADS>
+__device__ __forceinline__ bool find_run(const int32_t *__restrict__ off, int G, int M, int step, int wanted, bool typed,
+                                         Run *run)
+{
+    __shared__ Run found;
+    find_runs<THREADS>(off, G, M, step, typed, 1, [&](int) { return wanted; }, &found);
     *run = found;
-    return hit != 0;
+    return found.pieces != 0;
 }
 
 struct GroupedArgs {
@@ -162,6 +173,76 @@ template <typename T, typename S, Layout WL> __global__ __launch_bounds__(S::kTh
                 store4<T>(static_cast<T *>(a.out) + (int64_t)(row0 + m) * a.N + n, acc[i][j] + b, a.N - n, a.whole);
         }
     }
+}
+
+// The same with operands that stream into LDS (bfloat16, K and N multiples of 8, whole addresses).
+// Workgroup b has tiles first(b), first(b) + gridDim.x, ...: at most kRunsKept.  The tiles of a run's
+// columns are neighbours, and the workgroups of one XCD (every eighth) take neighbouring tiles: they
+// share rows of x and the weight of a type in one L2.
+constexpr int kRunsKept = 64;
+
+__device__ __forceinline__ int first_tile()
+{
+    const int g = gridDim.x, b = blockIdx.x;
+    return g % 8 == 0 ? (b % 8) * (g / 8) + b / 8 : b;
+}
+
+template <typename S, Layout WL> __global__ __launch_bounds__(S::kThreads, 2) void grouped_rows_stream(GroupedArgs a, int mtiles)
+{
+    using Product = StreamProduct<S, WL, kAlongK>;
+    extern __shared__ __align__(16) char lds[];
+    __shared__ Run runs[kRunsKept];
+    const int ntiles = (a.N + S::BN - 1) / S::BN;
+    const int first = first_tile(), tiles = mtiles * ntiles;
+    const int mine = first < tiles ? (tiles - 1 - first) / (int)gridDim.x + 1 : 0;
+    auto number = [&](int t) { return first + t * (int)gridDim.x; };
+    find_runs<S::kThreads>(a.off, a.G, a.M, S::BM, false, mine, [&](int t) { return number(t) / ntiles; }, runs);
+    int count = 0;      // pieces are numbered without gaps: those that exist come first
+    while (count < mine && uniform(runs[count].pieces) != 0) count++;
+    const bf16 *x = static_cast<const bf16 *>(a.x), *w = static_cast<const bf16 *>(a.w);
+    auto typed = [&](int type) { return type >= 0 && type < a.G; };
+    Product::template run<kNoSums>(
+        count, lds,
+        [&](int t) {
+            const int type = uniform(runs[t].type), row0 = uniform(runs[t].row), rows = uniform(runs[t].rows);
+            const int n0 = (number(t) % ntiles) * S::BN;
+            const bf16 *wt = w + (int64_t)(typed(type) ? type : 0) * a.K * a.N;
+            return StreamTile{WL == kAlongK ? wt + (int64_t)n0 * a.K : wt + n0, x + (int64_t)row0 * a.K, 0, 0,
+                              WL == kAlongK ? a.K : a.N, a.K, a.N - n0, rows, typed(type) ? a.K : 0};
+        },
+        [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *) {
+            const int type = uniform(runs[t].type), row0 = uniform(runs[t].row), rows = uniform(runs[t].rows);
+            const int n0 = (number(t) % ntiles) * S::BN;
+            constexpr int kRun = Product::kPairs ? 2 : 1;      // fragments whose results are neighbours
+#pragma unroll
+            for (int i = 0; i < S::FN; i += kRun) {
+                const int n = n0 + Product::n_of(i);
+                if (n >= a.N) continue;
+                f32x4 b[kRun];
+#pragma unroll
+                for (int u = 0; u < kRun; u++) {
+                    b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (a.bias && typed(type)) {
+                        const bf16 *src = static_cast<const bf16 *>(a.bias) + (int64_t)type * a.N + n + 4 * u;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) b[u][r] = to_float(src[r]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < S::FM; j++) {
+                    const int m = Product::m_of(j);
+                    if (m >= rows) continue;
+                    bf16 *out = static_cast<bf16 *>(a.out) + (int64_t)(row0 + m) * a.N + n;
+                    const f32x4 v = acc[i][j] + b[0];
+                    if constexpr (kRun == 2) {
+                        const f32x4 v2 = acc[i + 1][j] + b[1];
+                        *reinterpret_cast<u32x4 *>(out) = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
+                                                                pack_bf16(v2[0], v2[1]), pack_bf16(v2[2], v2[3])};
+                    } else
+                        *reinterpret_cast<u32x2 *>(out) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+                }
+            }
+        });
 }
 
 struct GradArgs {
@@ -218,58 +299,128 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads) void
     }
 }
 
-// Adds the pieces of the types that have several, in order.  grid: x = 1024 results each, y = types
+// The same, streaming
+template <typename S, Sums SUMS> __global__ __launch_bounds__(S::kThreads, 2) void grouped_weight_grad_stream(GradArgs a, int pieces)
+{
+    using Product = StreamProduct<S, kAcrossK, kAcrossK>;
+    extern __shared__ __align__(16) char lds[];
+    __shared__ Run runs[kRunsKept];
+    const int ntiles = (a.N + S::BN - 1) / S::BN, ktiles = (a.K + S::BM - 1) / S::BM, each = ntiles * ktiles;
+    const int first = first_tile(), tiles = pieces * each;
+    const int mine = first < tiles ? (tiles - 1 - first) / (int)gridDim.x + 1 : 0;
+    auto number = [&](int t) { return first + t * (int)gridDim.x; };
+    find_runs<S::kThreads>(a.off, a.G, a.M, a.piece, true, mine, [&](int t) { return number(t) / each; }, runs);
+    int count = 0;
+    while (count < mine && uniform(runs[count].pieces) != 0) count++;
+    const bf16 *x = static_cast<const bf16 *>(a.x), *dout = static_cast<const bf16 *>(a.dout);
+    auto corner = [&](int t, int *n0, int *k0) {
+        const int tile = number(t) % each;
+        *n0 = (tile % ntiles) * S::BN;
+        *k0 = (tile / ntiles) * S::BM;
+    };
+    Product::template run<SUMS>(
+        count, lds,
+        [&](int t) {
+            int n0, k0;
+            corner(t, &n0, &k0);
+            const int row0 = uniform(runs[t].row), rows = uniform(runs[t].rows);
+            return StreamTile{dout + (int64_t)row0 * a.N + n0, x + (int64_t)row0 * a.K + k0, 0, 0,
+                              a.N, a.K, a.N - n0, a.K - k0, rows};
+        },
+        [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *sums) {
+            int n0, k0;
+            corner(t, &n0, &k0);
+            const int type = uniform(runs[t].type);
+            const bool direct = uniform(runs[t].pieces) == 1;
+            const int64_t slot = (int64_t)uniform(runs[t].slot) + uniform(runs[t].piece);
+#pragma unroll
+            for (int i = 0; i < S::FN; i++) {
+                const int n = n0 + Product::n_of(i);
+                if (n >= a.N) continue;
+                if (SUMS == kSumP && k0 == 0 && Product::m_of(0) == 0) {
+                    if (direct) store4<bf16>(static_cast<bf16 *>(a.db) + (int64_t)type * a.N + n, sums[i], 4, a.whole);
+                    else store4<float>(a.part_b + slot * a.N + n, sums[i], 4, true);
+                }
+#pragma unroll
+                for (int j = 0; j < S::FM; j++) {
+                    const int k = k0 + Product::m_of(j);
+                    if (k >= a.K) continue;
+                    if (direct)
+                        store4<bf16>(static_cast<bf16 *>(a.dw) + ((int64_t)type * a.K + k) * a.N + n, acc[i][j], 4, a.whole);
+                    else store4<float>(a.part + (slot * a.K + k) * a.N + n, acc[i][j], 4, true);
+                }
+            }
+        });
+}
+
+// Adds the pieces of the types that have several, in order: workgroup y takes the y-th such type.
+// grid: x = results / 1024, y = as many such types as there can be
 template <typename T> __global__ __launch_bounds__(256) void grouped_weight_grad_sum(GradArgs a)
 {
-    __shared__ int s_pieces;
     __shared__ int wave_totals[4];
-    const int type = blockIdx.y;
-    // this type's pieces and the slots of the types before it, from offsets 0 .. type + 1
-    int totals_ignored;
-    const int n = type + 2;
+    __shared__ int s_type, s_slot, s_pieces;
+    const int n = a.G + 1;
     const int per = (n + 255) / 256;
     const int first = min((int)threadIdx.x * per, n), last = min(first + per, n);
     auto clean = [&](int i) { return min(max(a.off[i], 0), a.M); };
-    int top = 0;
+    int top = 0, ignored;
     for (int i = first; i < last; i++) top = max(top, clean(i));
-    const int before = block_exclusive<256, true>(top, wave_totals, &totals_ignored);
-    int slots = 0, mine = 0, begin = before, high = before;
-    for (int i = first; i < last; i++) {
-        high = max(high, clean(i));
-        const int np = i >= 1 && high > begin ? (high - begin - 1) / a.piece + 1 : 0;
-        if (i == type + 1) mine = np;
-        else slots += np > 1 ? np : 0;
-        begin = high;
-    }
-    int slots_before;
-    block_exclusive<256, false>(slots, wave_totals, &slots_before);
-    if (first <= type + 1 && type + 1 < last) s_pieces = mine;
+    const int before = block_exclusive<256, true>(top, wave_totals, &ignored);
+    // type i - 1 has the rows between offset i - 1 and offset i
+    auto each = [&](auto &&body) {
+        int begin = before, high = before;
+        for (int i = first; i < last; i++) {
+            high = max(high, clean(i));
+            const int np = i >= 1 && high > begin ? (high - begin - 1) / a.piece + 1 : 0;
+            if (np > 1) body(i - 1, np);
+            begin = high;
+        }
+    };
+    int types = 0, slots = 0;
+    each([&](int, int np) {
+        types++;
+        slots += np;
+    });
+    int at = block_exclusive<256, false>(types, wave_totals, &ignored);
+    int slot_at = block_exclusive<256, false>(slots, wave_totals, &ignored);
+    if (threadIdx.x == 0) s_pieces = 0;
+    __syncthreads();
+    each([&](int type, int np) {
+        if (at++ == (int)blockIdx.y) {
+            s_type = type;
+            s_slot = slot_at;
+            s_pieces = np;
+        }
+        slot_at += np;
+    });
     __syncthreads();
     const int pieces = uniform(s_pieces);
-    if (pieces <= 1) return;
-    const int64_t slot = slots_before, size = (int64_t)a.K * a.N;
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const int64_t e = (int64_t)blockIdx.x * 1024 + u * 256 + threadIdx.x;
-        if (e < size) {
-            float v = 0.f;
-            for (int p = 0; p < pieces; p++) v += a.part[(slot + p) * size + e];
-            static_cast<T *>(a.dw)[type * size + e] = from_float<T>(v);
+    if (pieces == 0) return;
+    const int64_t type = uniform(s_type), slot = uniform(s_slot), size = (int64_t)a.K * a.N;
+    // four neighbouring results a thread, eight pieces under way at a time
+    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    auto add = [&](const float *part, int64_t stride, int64_t at, int n, T *out) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (n >= 4 && stride % 4 == 0) {
+            const f32x4 *src = reinterpret_cast<const f32x4 *>(part + slot * stride + at);
+#pragma unroll 8
+            for (int p = 0; p < pieces; p++) v += src[p * (stride / 4)];
+        } else {
+            for (int r = 0; r < 4 && r < n; r++)
+                for (int p = 0; p < pieces; p++) v[r] += part[(slot + p) * stride + at + r];
         }
-        if (a.db && e < a.N) {
-            float v = 0.f;
-            for (int p = 0; p < pieces; p++) v += a.part_b[(slot + p) * a.N + e];
-            static_cast<T *>(a.db)[(int64_t)type * a.N + e] = from_float<T>(v);
-        }
-    }
+        store4<T>(out + at, v, n, a.whole && stride % 4 == 0);
+    };
+    if (e < size) add(a.part, size, e, (int)min((int64_t)4, size - e), static_cast<T *>(a.dw) + type * size);
+    if (a.db && e < a.N) add(a.part_b, a.N, e, (int)min((int64_t)4, a.N - e), static_cast<T *>(a.db) + type * a.N);
 }
 
-// Rows a piece of the weight gradient sums: so many that about four workgroups per compute unit
+// Rows a piece of the weight gradient sums: so many that about three workgroups per compute unit
 // result, but whole steps of the product and at least 256
 static int grad_piece(int32_t M, int32_t K, int32_t N)
 {
     const int64_t tiles = ceil_div(K, 128) * ceil_div(N, 128);
-    const int64_t pieces = std::max<int64_t>(1, 1024 / tiles);
+    const int64_t pieces = std::max<int64_t>(1, 768 / tiles);
     const int64_t rows = ceil_div(ceil_div(M, pieces), 256) * 256;
     return (int)std::min<int64_t>(std::max<int64_t>(256, rows), 0x7fffff00);
 }
@@ -302,24 +453,62 @@ template <typename T, typename S, Layout WL> static int32_t launch_rows(const Gr
     return launch_status("grouped_rows");
 }
 
+// workgroups of a streaming launch: those resident at once, more only if one had over kRunsKept tiles
+template <typename S> static unsigned stream_grid(int64_t tiles)
+{
+    const int64_t resident = 256 * (160 * 1024 / S::kLds);
+    return (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(resident, ceil_div(ceil_div(tiles, kRunsKept), 8) * 8));
+}
+using RowsStream = StreamShape<1, 256, 128, 2, 2, 32, 3>;
+using GradStream = StreamShape<1, 256, 128, 2, 2, 32, 3>;
+
+template <Layout WL> static int32_t launch_rows_stream(const GroupedArgs &a, hipStream_t s)
+{
+    using S = RowsStream;
+    const int64_t mtiles = (int64_t)a.M / S::BM + std::min<int64_t>(a.G, a.M) + 2;
+    const int64_t tiles = mtiles * ceil_div(a.N, S::BN);
+    if (tiles > 0x3fffffffLL) return fail(JGAMD_ERR_SIZE, "grouped_rows: M=%d N=%d G=%d is too large", a.M, a.N, a.G);
+    raise_lds<&grouped_rows_stream<S, WL>>(S::kLds);
+    hipLaunchKernelGGL((grouped_rows_stream<S, WL>), dim3(stream_grid<S>(tiles)), dim3(S::kThreads), S::kLds, s, a, (int)mtiles);
+    return launch_status("grouped_rows");
+}
+
 template <typename T> static int32_t rows_of_type(const GroupedArgs &a, bool transposed, hipStream_t s)
 {
+    if (sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 &&
+        (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.out) & 15) == 0)
+        return transposed ? launch_rows_stream<kAlongK>(a, s) : launch_rows_stream<kAcrossK>(a, s);
     using S = Shape<T, 128, 128, 2, 2>;
     return transposed ? launch_rows<T, S, kAlongK>(a, s) : launch_rows<T, S, kAcrossK>(a, s);
 }
 
+template <Sums SUMS> static void launch_grad_stream(const GradArgs &a, int64_t pieces, int64_t tiles, hipStream_t s)
+{
+    using S = GradStream;
+    raise_lds<&grouped_weight_grad_stream<S, SUMS>>(S::kLds);
+    hipLaunchKernelGGL((grouped_weight_grad_stream<S, SUMS>), dim3(stream_grid<S>(tiles)), dim3(S::kThreads), S::kLds, s, a,
+                       (int)pieces);
+}
+
 template <typename T> static int32_t weight_grad_of_type(const GradArgs &a, hipStream_t s)
 {
-    using S = Shape<T, 128, 128, 2, 2>;
-    const int64_t tiles = ceil_div(a.N, S::BN) * ceil_div(a.K, S::BM);
-    const int64_t blocks = tiles * ((int64_t)a.M / a.piece + a.G);
-    if (blocks > 0x7fffffffLL)
+    const int64_t pieces = (int64_t)a.M / a.piece + a.G;
+    const bool stream = sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 && (((uintptr_t)a.x | (uintptr_t)a.dout) & 15) == 0;
+    const int bm = stream ? GradStream::BM : 128, bn = stream ? GradStream::BN : 128;
+    const int64_t tiles = ceil_div(a.N, bn) * ceil_div(a.K, bm) * pieces;
+    if (tiles > 0x3fffffffLL)
         return fail(JGAMD_ERR_SIZE, "grouped_rows_weight_grad: K=%d N=%d G=%d is too large", a.K, a.N, a.G);
-    hipLaunchKernelGGL((grouped_weight_grad<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, s, a);
+    if (stream) {
+        if (a.db) launch_grad_stream<kSumP>(a, pieces, tiles, s);
+        else launch_grad_stream<kNoSums>(a, pieces, tiles, s);
+    } else {
+        using S = Shape<T, 128, 128, 2, 2>;
+        hipLaunchKernelGGL((grouped_weight_grad<T, S>), dim3((unsigned)tiles), dim3(S::kThreads), 0, s, a);
+    }
     if (int32_t rc = launch_status("grouped_rows_weight_grad")) return rc;
     if (a.M <= a.piece) return 0;
     const unsigned gx = (unsigned)ceil_div((int64_t)a.K * a.N, 1024);
-    hipLaunchKernelGGL((grouped_weight_grad_sum<T>), dim3(gx, (unsigned)a.G), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((grouped_weight_grad_sum<T>), dim3(gx, (unsigned)std::min(a.G, a.M / a.piece)), dim3(256), 0, s, a);
     return launch_status("grouped_rows_weight_grad");
 }
 

@@ -27,16 +27,24 @@
 
 namespace jg {
 
-constexpr int kNormBlocks = 1024;      // workgroups of the backward pass, at most
+// Workgroups of the backward pass, at most: those resident at once (100 registers, 60 without a block).
+// 30011 rows of 1001 floats without a block: 92 us with 1024, 72 with 2048; 262144 rows of 1024 bfloat16
+// with one: 890 with 1024, 1040 with 2048.
+constexpr int kNormBlocks = 1024, kNormBlocksAlone = 2048;
 constexpr int kNormMaxWidth = 8192;
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);      // elements of a 16-byte access
+constexpr int kGradVec = 4;      // of the backward pass: eight arrays of a row in registers leave no room for more
 
-// V consecutive elements as floats; `n` of them exist (the rest read as zero, are not written)
-__device__ __forceinline__ void load_vec(const bf16 *p, int n, float (&v)[8])
+// V consecutive elements as floats; `n` of them exist (the rest read as zero, are not written).
+// WHOLE: rows are whole vectors, n is at least V or nothing exists.
+template <bool WHOLE> __device__ __forceinline__ void load_vec(const bf16 *p, int n, float (&v)[8])
 {
     Eight<bf16> e;
-    if (n >= 8) e.load(p);
+    if (WHOLE) {
+        e.clear();
+        if (n > 0) e.load(p);
+    } else if (n >= 8) e.load(p);
     else e.load_some(p, n);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -44,41 +52,92 @@ __device__ __forceinline__ void load_vec(const bf16 *p, int n, float (&v)[8])
         v[2 * i + 1] = bf16_hi(e.v[i]);
     }
 }
-__device__ __forceinline__ void load_vec(const float *p, int n, float (&v)[4])
-{
-    if (n >= 4) {
-        const f32x4 e = *reinterpret_cast<const f32x4_at4 *>(p);
+typedef uint32_t u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
+
+// four elements as they lie in memory, on their way to four floats
+template <typename T> struct Four;
+template <> struct Four<bf16> {
+    u32x2 v;
+    __device__ __forceinline__ void clear() { v = u32x2{0, 0}; }
+    __device__ __forceinline__ void load(const bf16 *p) { v = *reinterpret_cast<const u32x2_at2 *>(p); }
+    __device__ __forceinline__ void load_some(const bf16 *p, int n)
+    {
+        uint32_t e[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = e[i];
-    } else {
+        for (int i = 0; i < 4; i++) e[i] = i < n ? p[i].u : 0;
+        v = u32x2{e[0] | e[1] << 16, e[2] | e[3] << 16};
+    }
+    __device__ __forceinline__ void get(float (&f)[4]) const
+    {
+        f[0] = bf16_lo(v[0]), f[1] = bf16_hi(v[0]), f[2] = bf16_lo(v[1]), f[3] = bf16_hi(v[1]);
+    }
+};
+template <> struct Four<float> {
+    f32x4 v;
+    __device__ __forceinline__ void clear() { v = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ void load(const float *p) { v = *reinterpret_cast<const f32x4_at4 *>(p); }
+    __device__ __forceinline__ void load_some(const float *p, int n)
+    {
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = i < n ? p[i] : 0.f;
     }
-}
-__device__ __forceinline__ void store_vec(bf16 *p, int n, const float (&v)[8])
+    __device__ __forceinline__ void get(float (&f)[4]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = v[i];
+    }
+};
+template <bool WHOLE, typename T> __device__ __forceinline__ Four<T> load_four(const T *p, int n)
 {
-    if (n >= 8) {
+    Four<T> e;
+    if (WHOLE) {
+        e.clear();
+        if (n > 0) e.load(p);
+    } else if (n >= 4) e.load(p);
+    else e.load_some(p, n);
+    return e;
+}
+template <bool WHOLE, typename T> __device__ __forceinline__ void load_vec(const T *p, int n, float (&v)[4])
+{
+    load_four<WHOLE>(p, n).get(v);
+}
+template <bool WHOLE> __device__ __forceinline__ void store_vec(bf16 *p, int n, const float (&v)[4])
+{
+    if (WHOLE ? n > 0 : n >= 4) {
+        *reinterpret_cast<u32x2_at2 *>(p) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+        return;
+    }
+    if (WHOLE) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < n) p[i] = from_float<bf16>(v[i]);
+}
+template <bool WHOLE> __device__ __forceinline__ void store_vec(bf16 *p, int n, const float (&v)[8])
+{
+    if (WHOLE ? n > 0 : n >= 8) {
         *reinterpret_cast<u32x4_at2 *>(p) =
             u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
         return;
     }
+    if (WHOLE) return;
 #pragma unroll
     for (int i = 0; i < 8; i++)
         if (i < n) p[i] = from_float<bf16>(v[i]);
 }
-__device__ __forceinline__ void store_vec(float *p, int n, const float (&v)[4])
+template <bool WHOLE> __device__ __forceinline__ void store_vec(float *p, int n, const float (&v)[4])
 {
-    if (n >= 4) {
+    if (WHOLE ? n > 0 : n >= 4) {
         *reinterpret_cast<f32x4_at4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
         return;
     }
+    if (WHOLE) return;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (i < n) p[i] = v[i];
 }
 
-// sums of `v[0..N-1]` over the L lanes of a row, in every one of them.  L > 64: the row's lanes are
-// the workgroup, which calls this together; `scratch` holds N * L / 64 floats.
+// sums of `v[0..N-1]` over the L lanes of a row, in every one of them.  L > 64: the workgroup calls this
+// together; `scratch` holds N floats a wavefront.
 template <int L, int N> __device__ __forceinline__ void row_sum(float (&v)[N], float *scratch)
 {
 #pragma unroll
@@ -87,15 +146,17 @@ template <int L, int N> __device__ __forceinline__ void row_sum(float (&v)[N], f
         for (int o = (L < kWave ? L : kWave) / 2; o > 0; o >>= 1) v[i] += __shfl_xor(v[i], o, kWave);
     if (L > kWave) {
         constexpr int waves = L / kWave;
+        const int first = wave_in_block() / waves * waves;
         __syncthreads();
         if (lane_id() == 0)
 #pragma unroll
-            for (int i = 0; i < N; i++) scratch[i * waves + wave_in_block()] = v[i];
+            for (int i = 0; i < N; i++) scratch[wave_in_block() * N + i] = v[i];
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < N; i++) {
             v[i] = 0.f;
-            for (int w = 0; w < waves; w++) v[i] += scratch[i * waves + w];
+#pragma unroll
+            for (int w = 0; w < waves; w++) v[i] += scratch[(first + w) * N + i];
         }
     }
 }
@@ -109,15 +170,17 @@ struct NormArgs {
     float eps;
 };
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + __expf(-g)); }
+// hardware exponential and reciprocal: within a few units of the last place
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
 
 template <int L> constexpr int norm_threads() { return L > 256 ? L : 256; }
 
 // L lanes a row, C vectors a lane; grid: rows / (threads / L)
-template <typename T, int L, int C> __global__ __launch_bounds__(norm_threads<L>()) void norm_fwd(NormArgs a)
+template <typename T, int L, int C, bool WHOLE>
+__global__ __launch_bounds__(norm_threads<L>()) void norm_fwd(NormArgs a)
 {
     constexpr int V = kVec<T>;
-    __shared__ float scratch[2 * (L > kWave ? L / kWave : 1)];
+    __shared__ float scratch[2 * norm_threads<L>() / kWave];
     const int lane = threadIdx.x % L;
     const int64_t row = (int64_t)blockIdx.x * (norm_threads<L>() / L) + threadIdx.x / L;
     const bool mine = row < a.R;      // rows past the last are computed from nothing and not stored
@@ -130,9 +193,9 @@ template <typename T, int L, int C> __global__ __launch_bounds__(norm_threads<L>
     for (int c = 0; c < C; c++) {
         const int f = (c * L + lane) * V;
         left[c] = mine ? a.F - f : 0;
-        load_vec(x + base + f, left[c], s[c]);
-        if (y) load_vec(y + base + f, left[c], b[c]);
-        if (gate) load_vec(gate + base + f, left[c], q[c]);
+        load_vec<WHOLE>(x + base + f, left[c], s[c]);
+        if (y) load_vec<WHOLE>(y + base + f, left[c], b[c]);
+        if (gate) load_vec<WHOLE>(gate + base + f, left[c], q[c]);
     }
     if (y) {
         float ry = 1.f;
@@ -151,7 +214,7 @@ template <typename T, int L, int C> __global__ __launch_bounds__(norm_threads<L>
             const int f = (c * L + lane) * V;
             float v[V];
             if (post) {
-                load_vec(post + f, left[c], v);
+                load_vec<WHOLE>(post + f, left[c], v);
 #pragma unroll
                 for (int i = 0; i < V; i++) b[c][i] *= ry * v[i];
             }
@@ -160,13 +223,13 @@ template <typename T, int L, int C> __global__ __launch_bounds__(norm_threads<L>
                 for (int i = 0; i < V; i++) b[c][i] *= sigmoid(q[c][i]);
             }
             if (scale) {
-                load_vec(scale + f, left[c], v);
+                load_vec<WHOLE>(scale + f, left[c], v);
 #pragma unroll
                 for (int i = 0; i < V; i++) b[c][i] *= v[i];
             }
 #pragma unroll
             for (int i = 0; i < V; i++) s[c][i] += i < left[c] ? b[c][i] : 0.f;
-            if (a.s) store_vec(static_cast<T *>(a.s) + base + f, left[c], s[c]);
+            if (a.s) store_vec<WHOLE>(static_cast<T *>(a.s) + base + f, left[c], s[c]);
         }
     }
     float sum[1] = {0.f};
@@ -174,17 +237,17 @@ template <typename T, int L, int C> __global__ __launch_bounds__(norm_threads<L>
     for (int c = 0; c < C; c++)
 #pragma unroll
         for (int i = 0; i < V; i++) sum[0] += s[c][i] * s[c][i];
-    row_sum<L>(sum, scratch + (L > kWave ? L / kWave : 1));
+    row_sum<L>(sum, scratch + norm_threads<L>() / kWave);
     const float rs = rsqrtf(sum[0] / (float)a.F + a.eps);
     if (a.rs && lane == 0 && mine) a.rs[row] = rs;
 #pragma unroll
     for (int c = 0; c < C; c++) {
         const int f = (c * L + lane) * V;
         float v[V];
-        load_vec(w + f, left[c], v);
+        load_vec<WHOLE>(w + f, left[c], v);
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] *= s[c][i] * rs;
-        store_vec(static_cast<T *>(a.h) + base + f, left[c], v);
+        store_vec<WHOLE>(static_cast<T *>(a.h) + base + f, left[c], v);
     }
 }
 
@@ -198,91 +261,143 @@ struct NormGradArgs {
     int F;
 };
 
-template <typename T, int L, int C> __global__ __launch_bounds__(norm_threads<L>()) void norm_bwd(NormGradArgs a)
+// BLOCK: there is a y.  grid: x = workgroups, each with every gridDim.x-th group of rows
+template <typename T, int L, int C, bool WHOLE, bool BLOCK>
+__global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(NormGradArgs a)
 {
-    constexpr int V = kVec<T>;
+    constexpr int V = kGradVec;
     constexpr int groups = norm_threads<L>() / L;      // rows of a workgroup at a time
-    __shared__ float scratch[3 * (L > kWave ? L / kWave : 1)];
+    __shared__ float scratch[3 * norm_threads<L>() / kWave];
     __shared__ float joined[groups > 1 ? norm_threads<L>() * C * V : 1];
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
-    const T *x = static_cast<const T *>(a.x), *y = static_cast<const T *>(a.y), *gate = static_cast<const T *>(a.gate);
-    const T *scale = static_cast<const T *>(a.scale), *post = static_cast<const T *>(a.post), *w = static_cast<const T *>(a.w);
+    const T *x = static_cast<const T *>(a.x), *y = BLOCK ? static_cast<const T *>(a.y) : nullptr;
+    const T *gate = BLOCK ? static_cast<const T *>(a.gate) : nullptr;
+    const T *scale = BLOCK ? static_cast<const T *>(a.scale) : nullptr, *post = BLOCK ? static_cast<const T *>(a.post) : nullptr;
+    const T *w = static_cast<const T *>(a.w);
     const T *ds = static_cast<const T *>(a.ds), *dh = static_cast<const T *>(a.dh);
     float sum_w[C][V] = {}, sum_p[C][V] = {}, sum_s[C][V] = {};
+    // the three small rows; a part that is left out counts as 1: no branch in the arithmetic
+    constexpr bool kKeep = C < 4;      // in registers, or read again for every row
+    struct Small {
+        float w[V], post[V], scale[V];
+    };
+    auto small = [&](int c) {
+        Small v;
+        const int f = (c * L + lane) * V, n = a.F - f;
+        load_vec<WHOLE>(w + f, n, v.w);
+        if (post) load_vec<WHOLE>(post + f, n, v.post);
+        if (scale) load_vec<WHOLE>(scale + f, n, v.scale);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            if (!post) v.post[i] = 1.f;
+            if (!scale) v.scale[i] = 1.f;
+        }
+        return v;
+    };
+    Small kept[kKeep ? C : 1];
+    if (kKeep)
+#pragma unroll
+        for (int c = 0; c < C; c++) kept[c] = small(c);
     const float over_f = 1.f / (float)a.F;
-    // every wavefront takes the same number of turns: the reductions of wide rows have barriers
-    for (int64_t row0 = (int64_t)blockIdx.x * groups; row0 < a.R; row0 += (int64_t)gridDim.x * groups) {
-        const int64_t row = row0 + group;
+    struct Row {
+        Four<T> x[C], y[C], gate[C], dh[C], ds[C];
+        float rs, ry;
+    };
+    auto read = [&](int64_t row) {
+        Row r;
         const bool mine = row < a.R;
         const int64_t base = row * a.F;
-        const float rs = mine ? a.rs[row] : 0.f, ry = mine && y && post ? a.ry[row] : 1.f;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int f = (c * L + lane) * V, left = mine ? a.F - f : 0;
+            r.x[c] = load_four<WHOLE>(x + base + f, left);
+            r.y[c].clear();
+            r.gate[c].clear();
+            r.dh[c].clear();
+            r.ds[c].clear();
+            if (y) r.y[c] = load_four<WHOLE>(y + base + f, left);
+            if (gate) r.gate[c] = load_four<WHOLE>(gate + base + f, left);
+            if (dh) r.dh[c] = load_four<WHOLE>(dh + base + f, left);
+            if (ds) r.ds[c] = load_four<WHOLE>(ds + base + f, left);
+        }
+        r.rs = mine ? a.rs[row] : 0.f;
+        r.ry = mine && post ? a.ry[row] : 1.f;
+        return r;
+    };
+    // every wavefront takes the same number of turns: the reductions of wide rows have barriers.  What a
+    // lane holds past the row's end, or past the last row, is zero and adds zero.  The next row is read
+    // while this one is worked on (rows of 1024 bfloat16: 1192 -> 896 us for 262144 of them), but not
+    // where that costs more than it brings: rows with a ragged end (1001 floats: 78 us without, 97 with)
+    // and the widest, whose registers would spill.
+    constexpr bool kAhead = WHOLE && C < 4;
+    const int64_t stride = (int64_t)gridDim.x * groups;
+    Row next = read((int64_t)blockIdx.x * groups + group);
+    for (int64_t row0 = (int64_t)blockIdx.x * groups; row0 < a.R; row0 += stride) {
+        const int64_t row = row0 + group;
+        const int64_t base = row * a.F;
+        const float rs = next.rs, ry = next.ry;
         float s[C][V], b[C][V], t[C][V], g[C][V], e[C][V];
         int left[C];
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            const int f = (c * L + lane) * V;
-            left[c] = mine ? a.F - f : 0;
-            load_vec(x + base + f, left[c], s[c]);
-            if (y) load_vec(y + base + f, left[c], b[c]);
-            if (gate) load_vec(gate + base + f, left[c], g[c]);
-            if (dh) load_vec(dh + base + f, left[c], e[c]);
-            if (ds) load_vec(ds + base + f, left[c], t[c]);
+            left[c] = row < a.R ? a.F - (c * L + lane) * V : 0;
+            next.x[c].get(s[c]);
+            next.y[c].get(b[c]);
+            next.gate[c].get(g[c]);
+            next.dh[c].get(e[c]);
+            next.ds[c].get(t[c]);
         }
+        if (kAhead && row0 + stride < a.R) next = read(row + stride);
         float sums[3] = {0.f, 0.f, 0.f};      // dh w s, t q post y, s q post y
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            const int f = (c * L + lane) * V;
-            float wv[V], pv[V], sv[V];
-            load_vec(w + f, left[c], wv);
-            if (post) load_vec(post + f, left[c], pv);
-            if (scale) load_vec(scale + f, left[c], sv);
+            const Small k = kKeep ? kept[c] : small(c);
+            if (gate) {      // never without a block
+#pragma unroll
+                for (int i = 0; i < V; i++) g[c][i] = sigmoid(g[c][i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) g[c][i] = 1.f;
+            }
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const bool in = i < left[c];
-                if (y) {
-                    const float p = post ? pv[i] : 1.f, k = scale ? sv[i] : 1.f;
-                    g[c][i] = gate ? sigmoid(g[c][i]) : 1.f;
-                    s[c][i] += in ? k * g[c][i] * (b[c][i] * ry * p) : 0.f;
-                }
-                if (!dh) e[c][i] = 0.f;
-                if (!ds) t[c][i] = 0.f;
-                const float hw = e[c][i] * wv[i];
+                const float z = BLOCK ? k.scale[i] * g[c][i] * k.post[i] * b[c][i] : 0.f;
+                if (BLOCK) s[c][i] += z * ry;
+                const float hw = e[c][i] * k.w[i];
                 t[c][i] += rs * hw;
                 sums[0] += hw * s[c][i];
-                if (dh) sum_w[c][i] += e[c][i] * (s[c][i] * rs);
-                if (y && post) {
-                    const float z = (scale ? sv[i] : 1.f) * g[c][i] * pv[i] * b[c][i];
-                    sums[1] += in ? t[c][i] * z : 0.f;
-                    sums[2] += in ? s[c][i] * z : 0.f;
+                if (BLOCK) {
+                    sums[1] += t[c][i] * z;
+                    sums[2] += s[c][i] * z;
                 }
+                sum_w[c][i] += e[c][i] * (s[c][i] * rs);
             }
         }
-        row_sum<L>(sums, scratch);
+        if (BLOCK) row_sum<L>(sums, scratch);
+        else row_sum<L>(reinterpret_cast<float(&)[1]>(sums), scratch);
         const float back = rs * rs * rs * (sums[0] * over_f);
-        const float back_y = ry * ry * ry * ((sums[1] - back * sums[2]) * over_f);
+        const float back_y = post ? ry * ry * ry * ((sums[1] - back * sums[2]) * over_f) : 0.f;
 #pragma unroll
         for (int c = 0; c < C; c++) {
+            const Small k = kKeep ? kept[c] : small(c);
             const int f = (c * L + lane) * V;
-            float pv[V], sv[V], dy[V], dg[V];
-            if (post) load_vec(post + f, left[c], pv);
-            if (scale) load_vec(scale + f, left[c], sv);
+            float dy[V], dg[V];
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float dx = t[c][i] - s[c][i] * back;
                 t[c][i] = dx;
-                if (y) {
-                    const float k = scale ? sv[i] : 1.f, p = post ? pv[i] : 1.f;
-                    const float u = b[c][i] * ry, dv = dx * k * g[c][i];
-                    dy[i] = post ? ry * (dv * p) - b[c][i] * back_y : dv;
-                    dg[i] = dv * (u * p) * (1.f - g[c][i]);
-                    if (post) sum_p[c][i] += dv * u;
-                    if (scale) sum_s[c][i] += dx * g[c][i] * (u * p);
-                }
+                if (!BLOCK) continue;
+                const float u = b[c][i] * ry, xg = dx * g[c][i], dv = xg * k.scale[i], up = u * k.post[i];
+                dy[i] = ry * (dv * k.post[i]) - b[c][i] * back_y;
+                dg[i] = dv * up * (1.f - g[c][i]);
+                sum_p[c][i] += dv * u;
+                sum_s[c][i] += xg * up;
             }
-            if (a.dx) store_vec(static_cast<T *>(a.dx) + base + f, left[c], t[c]);
-            if (a.dy) store_vec(static_cast<T *>(a.dy) + base + f, left[c], dy);
-            if (a.dgate) store_vec(static_cast<T *>(a.dgate) + base + f, left[c], dg);
+            if (a.dx) store_vec<WHOLE>(static_cast<T *>(a.dx) + base + f, left[c], t[c]);
+            if (BLOCK && a.dy) store_vec<WHOLE>(static_cast<T *>(a.dy) + base + f, left[c], dy);
+            if (BLOCK && a.dgate) store_vec<WHOLE>(static_cast<T *>(a.dgate) + base + f, left[c], dg);
         }
+        if (!kAhead && row0 + stride < a.R) next = read(row + stride);
     }
     // the workgroup's column sums: its row groups in order
     auto join = [&](float (&v)[C][V], int which) {
@@ -308,58 +423,63 @@ template <typename T, int L, int C> __global__ __launch_bounds__(norm_threads<L>
         }
     };
     if (a.dw) join(sum_w, 0);
-    if (a.dpost) join(sum_p, 1);
-    if (a.dscale) join(sum_s, 2);
+    if (BLOCK && a.dpost) join(sum_p, 1);
+    if (BLOCK && a.dscale) join(sum_s, 2);
 }
 
-// The workgroups' sums in order: a workgroup adds 32 columns, 8 strands of workgroups each.
+// The workgroups' sums in order: a workgroup adds 32 columns, 32 strands of workgroups each.
 // grid: x = columns / 32, y = the three sums
-template <typename T> __global__ __launch_bounds__(256) void norm_bwd_columns(NormGradArgs a, int blocks)
+template <typename T> __global__ __launch_bounds__(1024) void norm_bwd_columns(NormGradArgs a, int blocks)
 {
-    __shared__ float strands[8][32];
+    __shared__ float strands[32][33];
     void *out = blockIdx.y == 0 ? a.dw : blockIdx.y == 1 ? a.dpost : a.dscale;
     if (!out) return;
-    const int f = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
+    const int column = threadIdx.x & 31, strand = threadIdx.x >> 5;
+    const int f = blockIdx.x * 32 + column;
+    const float *part = a.part + (int64_t)blockIdx.y * blocks * a.F + f;
     float v = 0.f;
-    if (f < a.F)
-        for (int b = strand; b < blocks; b += 8) v += a.part[((int64_t)blockIdx.y * blocks + b) * a.F + f];
-    strands[strand][threadIdx.x & 31] = v;
+    if (f < a.F) {
+#pragma unroll 8
+        for (int b = strand; b < blocks; b += 32) v += part[(int64_t)b * a.F];
+    }
+    strands[strand][column] = v;
     __syncthreads();
     if (strand == 0 && f < a.F) {
 #pragma unroll
-        for (int k = 1; k < 8; k++) v += strands[k][threadIdx.x];
+        for (int k = 1; k < 32; k++) v += strands[k][column];
         static_cast<T *>(out)[f] = from_float<T>(v);
     }
 }
 
 // calls body(L, C) as compile-time constants: the narrowest lanes and vectors that cover a row
-template <typename T, typename Body> static void norm_shape(int F, Body &&body)
+template <int V, typename Body> static void norm_shape(int F, Body &&body)
 {
-    const int v = (int)ceil_div(F, kVec<T>);      // vectors of a row
+    const int v = (int)ceil_div(F, V);      // vectors of a row
     if (v <= 8) body(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
     else if (v <= 16) body(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
     else if (v <= 32) body(std::integral_constant<int, 32>(), std::integral_constant<int, 1>());
     else if (v <= 64) body(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-    else if (v <= 128) body(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    else if (v <= 128) body(std::integral_constant<int, 128>(), std::integral_constant<int, 1>());
     else if (v <= 256) body(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
     else if (v <= 512) body(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
     else if (v <= 1024) body(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
-    else if constexpr (kNormMaxWidth / kVec<T> > 1024)
+    else if constexpr (kNormMaxWidth / V > 1024)
         body(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
 }
-static int norm_lanes(int32_t dtype, int F)
+static int norm_grad_lanes(int F)
 {
     int lanes = 0;
-    auto take = [&](auto l, auto) { lanes = l; };
-    if (dtype == JGAMD_F32) norm_shape<float>(F, take);
-    else norm_shape<bf16>(F, take);
+    norm_shape<kGradVec>(F, [&](auto l, auto) { lanes = l; });
     return lanes;
 }
-static int norm_blocks(int64_t R, int lanes)
+static int norm_blocks(int64_t R, int lanes, bool block)
 {
     const int groups = lanes > 256 ? 1 : 256 / lanes;
-    return (int)std::min<int64_t>(ceil_div(R, groups), kNormBlocks);
+    return (int)std::min<int64_t>(ceil_div(R, groups), block ? kNormBlocks : kNormBlocksAlone);
 }
+
+// three sums of kNormBlocks workgroups, or one (and two unused) of kNormBlocksAlone
+static size_t norm_part_floats(int64_t R, int F) { return (size_t)3 * std::min<int64_t>(R, kNormBlocks) * F; }
 
 static int32_t norm_check(const char *who, int64_t R, int32_t F, int32_t dtype)
 {
@@ -393,10 +513,12 @@ JG_EXPORT int32_t jgamd_residual_norm_fwd(const void *x, const void *y, const vo
     auto launch = [&](auto type, auto l, auto c) {
         using T = decltype(type);
         constexpr int L = decltype(l)::value, C = decltype(c)::value, threads = norm_threads<L>();
-        hipLaunchKernelGGL((norm_fwd<T, L, C>), dim3((unsigned)ceil_div(R, threads / L)), dim3(threads), 0, st, a);
+        const dim3 grid((unsigned)ceil_div(R, threads / L));
+        if (F % kVec<T> == 0) hipLaunchKernelGGL((norm_fwd<T, L, C, true>), grid, dim3(threads), 0, st, a);
+        else hipLaunchKernelGGL((norm_fwd<T, L, C, false>), grid, dim3(threads), 0, st, a);
     };
-    if (dtype == JGAMD_F32) norm_shape<float>(F, [&](auto l, auto c) { launch(float(), l, c); });
-    else norm_shape<bf16>(F, [&](auto l, auto c) { launch(bf16(), l, c); });
+    if (dtype == JGAMD_F32) norm_shape<kVec<float>>(F, [&](auto l, auto c) { launch(float(), l, c); });
+    else norm_shape<kVec<bf16>>(F, [&](auto l, auto c) { launch(bf16(), l, c); });
     return launch_status("residual_norm_fwd");
 }
 
@@ -404,7 +526,7 @@ JG_EXPORT int32_t jgamd_residual_norm_bwd_workspace(int64_t R, int32_t F, size_t
 {
     if (!bytes) return fail(JGAMD_ERR_NULL, "residual_norm_bwd_workspace: bytes is NULL");
     if (int32_t rc = norm_check("residual_norm_bwd_workspace", R, F, JGAMD_F32)) return rc;
-    *bytes = carve_bytes((size_t)3 * std::min<int64_t>(R, kNormBlocks) * F, 4);
+    *bytes = carve_bytes(norm_part_floats(R, F), 4);
     return 0;
 }
 
@@ -426,7 +548,7 @@ JG_EXPORT int32_t jgamd_residual_norm_bwd(const void *x, const void *y, const vo
     if ((any & (dtype == JGAMD_F32 ? 3 : 1)) || (((uintptr_t)ry | (uintptr_t)rs) & 3))
         return fail(JGAMD_ERR_ALIGN, "residual_norm_bwd: an array does not start at a multiple of its element's size");
     const bool columns = dw || dpost || dscale;
-    const size_t need = columns ? carve_bytes((size_t)3 * std::min<int64_t>(R, kNormBlocks) * F, 4) : 0;
+    const size_t need = columns ? carve_bytes(norm_part_floats(R, F), 4) : 0;
     if (need > 0 && (!ws || ws_bytes < need))
         return fail(JGAMD_ERR_WORKSPACE, "residual_norm_bwd: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, need);
     if (need > 0 && ((uintptr_t)ws & 255) != 0)
@@ -434,20 +556,27 @@ JG_EXPORT int32_t jgamd_residual_norm_bwd(const void *x, const void *y, const vo
     const NormGradArgs a{x, y, gate, scale, post, w, ry, rs, ds, dh, dx, dy, dgate, dscale, dpost, dw,
                          static_cast<float *>(ws), R, F};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int blocks = norm_blocks(R, norm_lanes(dtype, F));
+    const int blocks = norm_blocks(R, norm_grad_lanes(F), y != nullptr);
     auto launch = [&](auto type, auto l, auto c) {
         using T = decltype(type);
         constexpr int L = decltype(l)::value, C = decltype(c)::value;
-        hipLaunchKernelGGL((norm_bwd<T, L, C>), dim3((unsigned)blocks), dim3(norm_threads<L>()), 0, st, a);
+        const dim3 grid((unsigned)blocks), threads(norm_threads<L>());
+        if (F % kGradVec == 0) {
+            if (y) hipLaunchKernelGGL((norm_bwd<T, L, C, true, true>), grid, threads, 0, st, a);
+            else hipLaunchKernelGGL((norm_bwd<T, L, C, true, false>), grid, threads, 0, st, a);
+        } else {
+            if (y) hipLaunchKernelGGL((norm_bwd<T, L, C, false, true>), grid, threads, 0, st, a);
+            else hipLaunchKernelGGL((norm_bwd<T, L, C, false, false>), grid, threads, 0, st, a);
+        }
     };
     if (blocks > 0) {
-        if (dtype == JGAMD_F32) norm_shape<float>(F, [&](auto l, auto c) { launch(float(), l, c); });
-        else norm_shape<bf16>(F, [&](auto l, auto c) { launch(bf16(), l, c); });
+        if (dtype == JGAMD_F32) norm_shape<kGradVec>(F, [&](auto l, auto c) { launch(float(), l, c); });
+        else norm_shape<kGradVec>(F, [&](auto l, auto c) { launch(bf16(), l, c); });
         if (int32_t rc = launch_status("residual_norm_bwd")) return rc;
     }
     if (!columns) return 0;
     const dim3 grid((unsigned)ceil_div(F, 32), 3);
-    if (dtype == JGAMD_F32) hipLaunchKernelGGL((norm_bwd_columns<float>), grid, dim3(256), 0, st, a, blocks);
-    else hipLaunchKernelGGL((norm_bwd_columns<bf16>), grid, dim3(256), 0, st, a, blocks);
+    if (dtype == JGAMD_F32) hipLaunchKernelGGL((norm_bwd_columns<float>), grid, dim3(1024), 0, st, a, blocks);
+    else hipLaunchKernelGGL((norm_bwd_columns<bf16>), grid, dim3(1024), 0, st, a, blocks);
     return launch_status("residual_norm_bwd");
 }
