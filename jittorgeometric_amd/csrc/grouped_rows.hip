@@ -245,6 +245,138 @@ template <typename S, Layout WL> __global__ __launch_bounds__(S::kThreads, 2) vo
         });
 }
 
+// Few rows: the weights are read once and multiplied on the vector unit.  A tile of 128 rows holds a
+// handful, its steps follow one another a memory latency each, and reading the weights is all there is
+// to do: here every wavefront asks for its share of them at once.  kThinRows rows of x stand in LDS as
+// floats.  48 rows of 16 types, 256 x 256 floats: 20.6 us with tiles, 6 like this.
+constexpr int kThinRows = 8;
+constexpr int kThinMost = 128;       // rows of a call, at most
+constexpr int kThinSteps = 512;      // of k in LDS at a time
+constexpr int kThinThreads = 512;
+
+// rows row0 .. row0 + rows - 1 of x, steps k0 .. k0 + kThinSteps - 1, zero where there is none
+template <typename T>
+__device__ __forceinline__ void thin_stage(const T *x, int row0, int rows, int K, int k0, float (*xs)[kThinSteps])
+{
+#pragma unroll
+    for (int r = 0; r < kThinRows; r++) {
+        const int k = k0 + threadIdx.x;
+        xs[r][threadIdx.x] = r < rows && k < K ? to_float(x[(int64_t)(row0 + r) * K + k]) : 0.f;
+    }
+}
+static_assert(kThinSteps == kThinThreads, "a thread stages one step of every row");
+
+// W [K][N]: two neighbouring columns a lane, CW columns a workgroup; wavefronts and the lanes that
+// columns leave over share k.  grid: x = runs x blocks of CW columns
+template <typename T, int CW> __global__ __launch_bounds__(kThinThreads) void grouped_thin_across(GroupedArgs a)
+{
+    constexpr int kLanes = CW / 2, kShares = kThinThreads / kLanes;      // lanes of a step, steps at a time
+    __shared__ float xs[kThinRows][kThinSteps];
+    __shared__ float part[kShares / 2][kThinRows][CW];
+    const int blocks = (a.N + CW - 1) / CW;
+    Run run;
+    if (!find_run<kThinThreads>(a.off, a.G, a.M, kThinRows, blockIdx.x / blocks, false, &run)) return;
+    const int type = uniform(run.type), row0 = uniform(run.row), rows = uniform(run.rows);
+    const bool typed = type >= 0 && type < a.G;
+    const int col = (blockIdx.x % blocks) * CW + (threadIdx.x % kLanes) * 2, share = threadIdx.x / kLanes;
+    const int n = a.N - col;      // columns from here on
+    float acc[kThinRows][2] = {};
+    if (typed) {
+        const T *w = static_cast<const T *>(a.w) + (int64_t)type * a.K * a.N + (n > 0 ? col : 0);
+        for (int k0 = 0; k0 < a.K; k0 += kThinSteps) {
+            __syncthreads();
+            thin_stage(static_cast<const T *>(a.x), row0, rows, a.K, k0, xs);
+            __syncthreads();
+            const int steps = min(kThinSteps, a.K - k0);
+#pragma unroll 8
+            for (int k = share; k < steps; k += kShares) {
+                const T *src = w + (int64_t)(k0 + k) * a.N;
+                const float w0 = to_float(src[0]), w1 = to_float(src[n > 1 ? 1 : 0]);
+#pragma unroll
+                for (int r = 0; r < kThinRows; r++) {
+                    const float xv = xs[r][k];
+                    acc[r][0] = fmaf(xv, w0, acc[r][0]);
+                    acc[r][1] = fmaf(xv, w1, acc[r][1]);
+                }
+            }
+        }
+    }
+    // the shares in order, the upper half onto the lower first
+    const int c = (threadIdx.x % kLanes) * 2;
+    if (share >= kShares / 2)
+#pragma unroll
+        for (int r = 0; r < kThinRows; r++) {
+            part[share - kShares / 2][r][c] = acc[r][0];
+            part[share - kShares / 2][r][c + 1] = acc[r][1];
+        }
+    __syncthreads();
+    if (share < kShares / 2)
+#pragma unroll
+        for (int r = 0; r < kThinRows; r++) {
+            part[share][r][c] += acc[r][0];
+            part[share][r][c + 1] += acc[r][1];
+        }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * CW; e += kThinThreads) {
+        const int r = e / CW, column = (blockIdx.x % blocks) * CW + e % CW;
+        if (column >= a.N) continue;
+        float v = a.bias && typed ? to_float(static_cast<const T *>(a.bias)[(int64_t)type * a.N + column]) : 0.f;
+#pragma unroll
+        for (int s = 0; s < kShares / 2; s++) v += part[s][r][e % CW];
+        static_cast<T *>(a.out)[(int64_t)(row0 + r) * a.N + column] = from_float<T>(v);
+    }
+}
+
+// W [N][K]: sixteen lanes a row of W, 16 bytes each, whose sums meet in shuffles.
+// grid: x = runs x blocks of 32 columns
+template <typename T> __global__ __launch_bounds__(kThinThreads) void grouped_thin_along(GroupedArgs a)
+{
+    constexpr int V = 8, kColumns = kThinThreads / 16;
+    __shared__ __align__(16) float xs[kThinRows][kThinSteps];
+    const int blocks = (a.N + kColumns - 1) / kColumns;
+    Run run;
+    if (!find_run<kThinThreads>(a.off, a.G, a.M, kThinRows, blockIdx.x / blocks, false, &run)) return;
+    const int type = uniform(run.type), row0 = uniform(run.row), rows = uniform(run.rows);
+    const bool typed = type >= 0 && type < a.G;
+    const int lane = threadIdx.x % 16, col = (blockIdx.x % blocks) * kColumns + threadIdx.x / 16;
+    float acc[kThinRows] = {};
+    if (typed) {
+        const T *w = static_cast<const T *>(a.w) + ((int64_t)type * a.N + min(col, a.N - 1)) * a.K;
+        for (int k0 = 0; k0 < a.K; k0 += kThinSteps) {
+            __syncthreads();
+            thin_stage(static_cast<const T *>(a.x), row0, rows, a.K, k0, xs);
+            __syncthreads();
+            const int steps = min(kThinSteps, a.K - k0);
+#pragma unroll
+            for (int u = 0; u < kThinSteps / (16 * V); u++) {
+                const int k = (u * 16 + lane) * V, left = steps - k;
+                if (left <= 0) continue;
+                float wv[V];
+                if (left >= V) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) wv[i] = to_float(w[k0 + k + i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i++) wv[i] = i < left ? to_float(w[k0 + k + i]) : 0.f;
+                }
+#pragma unroll
+                for (int r = 0; r < kThinRows; r++)
+#pragma unroll
+                    for (int i = 0; i < V; i++) acc[r] = fmaf(xs[r][k + i], wv[i], acc[r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kThinRows; r++)
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) acc[r] += __shfl_xor(acc[r], o, 16);
+    if (lane != 0 || col >= a.N) return;
+    const float b = a.bias && typed ? to_float(static_cast<const T *>(a.bias)[(int64_t)type * a.N + col]) : 0.f;
+#pragma unroll
+    for (int r = 0; r < kThinRows; r++)
+        if (r < rows) static_cast<T *>(a.out)[(int64_t)(row0 + r) * a.N + col] = from_float<T>(acc[r] + b);
+}
+
 struct GradArgs {
     const void *x, *dout;
     const int32_t *off;
@@ -459,12 +591,14 @@ template <typename S> static unsigned stream_grid(int64_t tiles)
     const int64_t resident = 256 * (160 * 1024 / S::kLds);
     return (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(resident, ceil_div(ceil_div(tiles, kRunsKept), 8) * 8));
 }
-using RowsStream = StreamShape<1, 256, 128, 2, 2, 32, 3>;
-using GradStream = StreamShape<1, 256, 128, 2, 2, 32, 3>;
+// 256 x 128 results (two workgroups a compute unit, steps of 32) against 256 x 256 (one, steps of 64): 65521 rows,
+// 32 types, 1024 x 2048: 423 and 420 us against 380 and 358 (the two directions); 120011 rows, 256 x 256: 45, 38
+// against 42, 35
+using TypedStream = StreamShape<1, 256, 256, 2, 4, 64, 2>;
 
 template <Layout WL> static int32_t launch_rows_stream(const GroupedArgs &a, hipStream_t s)
 {
-    using S = RowsStream;
+    using S = TypedStream;
     const int64_t mtiles = (int64_t)a.M / S::BM + std::min<int64_t>(a.G, a.M) + 2;
     const int64_t tiles = mtiles * ceil_div(a.N, S::BN);
     if (tiles > 0x3fffffffLL) return fail(JGAMD_ERR_SIZE, "grouped_rows: M=%d N=%d G=%d is too large", a.M, a.N, a.G);
@@ -473,8 +607,21 @@ template <Layout WL> static int32_t launch_rows_stream(const GroupedArgs &a, hip
     return launch_status("grouped_rows");
 }
 
+template <typename T> static int32_t launch_thin(const GroupedArgs &a, bool transposed, hipStream_t s)
+{
+    const unsigned runs = a.M / kThinRows + std::min(a.G, a.M) + 2;
+    const unsigned wide = (unsigned)ceil_div(a.N, 128), narrow = (unsigned)ceil_div(a.N, 32);
+    if (transposed) hipLaunchKernelGGL((grouped_thin_along<T>), dim3(runs * narrow), dim3(kThinThreads), 0, s, a);
+    // 32 columns a workgroup where 128 would leave compute units without one
+    else if (runs * wide < 256) hipLaunchKernelGGL((grouped_thin_across<T, 32>), dim3(runs * narrow), dim3(kThinThreads), 0, s, a);
+    else hipLaunchKernelGGL((grouped_thin_across<T, 128>), dim3(runs * wide), dim3(kThinThreads), 0, s, a);
+    return launch_status("grouped_rows");
+}
+
 template <typename T> static int32_t rows_of_type(const GroupedArgs &a, bool transposed, hipStream_t s)
 {
+    // on average at most kThinRows rows a type; all of them of one type read its weight up to 16 times
+    if (a.M <= kThinMost && a.M <= (int64_t)kThinRows * a.G) return launch_thin<T>(a, transposed, s);
     if (sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 &&
         (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.out) & 15) == 0)
         return transposed ? launch_rows_stream<kAlongK>(a, s) : launch_rows_stream<kAcrossK>(a, s);
@@ -484,7 +631,7 @@ template <typename T> static int32_t rows_of_type(const GroupedArgs &a, bool tra
 
 template <Sums SUMS> static void launch_grad_stream(const GradArgs &a, int64_t pieces, int64_t tiles, hipStream_t s)
 {
-    using S = GradStream;
+    using S = TypedStream;
     raise_lds<&grouped_weight_grad_stream<S, SUMS>>(S::kLds);
     hipLaunchKernelGGL((grouped_weight_grad_stream<S, SUMS>), dim3(stream_grid<S>(tiles)), dim3(S::kThreads), S::kLds, s, a,
                        (int)pieces);
@@ -494,7 +641,7 @@ template <typename T> static int32_t weight_grad_of_type(const GradArgs &a, hipS
 {
     const int64_t pieces = (int64_t)a.M / a.piece + a.G;
     const bool stream = sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 && (((uintptr_t)a.x | (uintptr_t)a.dout) & 15) == 0;
-    const int bm = stream ? GradStream::BM : 128, bn = stream ? GradStream::BN : 128;
+    const int bm = stream ? TypedStream::BM : 128, bn = stream ? TypedStream::BN : 128;
     const int64_t tiles = ceil_div(a.N, bn) * ceil_div(a.K, bm) * pieces;
     if (tiles > 0x3fffffffLL)
         return fail(JGAMD_ERR_SIZE, "grouped_rows_weight_grad: K=%d N=%d G=%d is too large", a.K, a.N, a.G);
