@@ -122,8 +122,19 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+# the stream's handle without a Stream object around it, where this torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device):
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def needs_grad(*tensors):
+    """Whether a call with these inputs is recorded for a backward pass."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 class on:

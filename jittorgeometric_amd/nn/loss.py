@@ -71,24 +71,30 @@ def nll_loss(log_probs, target):
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}      # JGAMD_LOSS_NONE, JGAMD_LOSS_MEAN, JGAMD_LOSS_SUM
 
 
+def _linear_forward(x, weight, bias, target, reduction):
+    """(loss, lse, count)"""
+    lib = _lib.load()
+    dev = x.device
+    V, F = x.shape
+    C = weight.shape[0]
+    code = _lib.dtype_code(x.dtype)
+    loss = torch.empty((V,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+    count = torch.empty((), dtype=torch.int32, device=dev)
+    lse = torch.empty(V, dtype=torch.float32, device=dev)
+    nbytes = _lib.query(lib.jgamd_linear_cross_entropy_workspace, V, F, C, code, 0)
+    ws = _lib.workspace(nbytes, dev)
+    with _lib.on(dev):
+        _lib.check(lib.jgamd_linear_cross_entropy_fwd(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(target),
+                                                      1 if target.dtype == torch.int64 else 0, V, F, C, code, reduction,
+                                                      _lib.ptr(loss), _lib.ptr(count), _lib.ptr(lse), _lib.ptr(ws), nbytes,
+                                                      _lib.stream_ptr(dev)))
+    return loss, lse, count
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, reduction):
-        lib = _lib.load()
-        dev = x.device
-        V, F = x.shape
-        C = weight.shape[0]
-        code = _lib.dtype_code(x.dtype)
-        i64 = 1 if target.dtype == torch.int64 else 0
-        loss = torch.empty((V,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-        count = torch.empty((), dtype=torch.int32, device=dev)
-        lse = torch.empty(V, dtype=torch.float32, device=dev)
-        nbytes = _lib.query(lib.jgamd_linear_cross_entropy_workspace, V, F, C, code, 0)
-        ws = _lib.workspace(nbytes, dev)
-        with _lib.on(dev):
-            _lib.check(lib.jgamd_linear_cross_entropy_fwd(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(target),
-                                                          i64, V, F, C, code, reduction, _lib.ptr(loss), _lib.ptr(count),
-                                                          _lib.ptr(lse), _lib.ptr(ws), nbytes, _lib.stream_ptr(dev)))
+        loss, lse, count = _linear_forward(x, weight, bias, target, reduction)
         ctx.save_for_backward(x, weight, bias, target, lse, count)
         ctx.reduction = reduction
         return loss
@@ -148,5 +154,9 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
         if t is not None and t.dtype != x.dtype:
             raise _lib.JgamdError("linear_cross_entropy: %s is %s, x is %s" % (name, t.dtype, x.dtype))
     x, weight = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (x.contiguous(), weight.contiguous()))
-    return _LinearCrossEntropy.apply(x, weight, None if bias is None else bias.contiguous(), target.contiguous(),
-                                     _REDUCTIONS[reduction])
+    if bias is not None:
+        bias = bias.contiguous()
+    target = target.contiguous()
+    if not _lib.needs_grad(x, weight, bias):
+        return _linear_forward(x, weight, bias, target, _REDUCTIONS[reduction])[0]
+    return _LinearCrossEntropy.apply(x, weight, bias, target, _REDUCTIONS[reduction])

@@ -7,21 +7,26 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 
 
+def _forward(x, y, w, post, gate, scale, eps, for_backward):
+    """(s, h, ry, rs): s None without y, the inverse norms only for a backward pass."""
+    lib = _lib.load()
+    dev = x.device
+    R, F = x.shape
+    s = torch.empty_like(x) if y is not None else None
+    h = torch.empty_like(x)
+    rs = torch.empty(R, dtype=torch.float32, device=dev) if for_backward else None
+    ry = torch.empty(R, dtype=torch.float32, device=dev) if for_backward and post is not None else None
+    with _lib.on(dev):
+        _lib.check(lib.jgamd_residual_norm_fwd(_lib.ptr(x), _lib.ptr(y), _lib.ptr(gate), _lib.ptr(scale), _lib.ptr(post),
+                                               _lib.ptr(w), _lib.ptr(s), _lib.ptr(h), _lib.ptr(ry), _lib.ptr(rs), R, F, eps,
+                                               _lib.dtype_code(x.dtype), _lib.stream_ptr(dev)))
+    return s, h, ry, rs
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, w, post, gate, scale, eps):
-        lib = _lib.load()
-        dev = x.device
-        R, F = x.shape
-        s = torch.empty_like(x) if y is not None else None
-        h = torch.empty_like(x)
-        rs = torch.empty(R, dtype=torch.float32, device=dev)
-        ry = torch.empty(R, dtype=torch.float32, device=dev) if post is not None else None
-        with _lib.on(dev):
-            _lib.check(lib.jgamd_residual_norm_fwd(_lib.ptr(x), _lib.ptr(y), _lib.ptr(gate), _lib.ptr(scale),
-                                                   _lib.ptr(post), _lib.ptr(w), _lib.ptr(s), _lib.ptr(h), _lib.ptr(ry),
-                                                   _lib.ptr(rs), R, F, eps, _lib.dtype_code(x.dtype),
-                                                   _lib.stream_ptr(dev)))
+        s, h, ry, rs = _forward(x, y, w, post, gate, scale, eps, True)
         ctx.save_for_backward(x, y, w, post, gate, scale, ry, rs)
         ctx.set_materialize_grads(False)
         return h if y is None else (s, h)
@@ -67,6 +72,9 @@ def _apply(who, x, y, weight, post_weight, gate, scale, eps):
         raise _lib.JgamdError("%s: eps must not be negative, got %r" % (who, eps))
     x, y, weight, post_weight, gate, scale = (None if t is None else t.contiguous()
                                               for t in (x, y, weight, post_weight, gate, scale))
+    if not _lib.needs_grad(x, y, weight, post_weight, gate, scale):
+        s, h, _, _ = _forward(x, y, weight, post_weight, gate, scale, float(eps), False)
+        return h if y is None else (s, h)
     return _ResidualNorm.apply(x, y, weight, post_weight, gate, scale, float(eps))
 
 

@@ -81,5 +81,9 @@ def grouped_rows(x, weight, offsets, bias=None):
             raise _lib.JgamdError("grouped_rows: %s is %s, x is %s" % (name, t.dtype, x.dtype))
     if offsets.dtype == torch.int64:      # beyond int32 is past the last row anyway
         offsets = offsets.clamp(0, 2**31 - 1).to(torch.int32)
-    return _GroupedRows.apply(x.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(),
-                              offsets.detach().contiguous())
+    x, weight, offsets = x.contiguous(), weight.contiguous(), offsets.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    if not _lib.needs_grad(x, weight, bias):
+        return _product(x, weight, bias, offsets, False)
+    return _GroupedRows.apply(x, weight, bias, offsets)
