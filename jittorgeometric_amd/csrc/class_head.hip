@@ -40,6 +40,15 @@ template <> struct HeadShapeOf<float> {
     using S = StreamShape<3, 256, 128, 4, 2, 32, 2>;
 };
 template <typename T> using HeadShape = typename HeadShapeOf<T>::S;
+// the forward pass of a few rows: all of w streams past one tile of them, two workgroups a compute unit
+template <typename T> struct HeadFewOf;
+template <> struct HeadFewOf<bf16> {
+    using S = StreamShape<1, 128, 32, 4, 1, 64, 4>;
+};
+template <> struct HeadFewOf<float> {
+    using S = StreamShape<3, 128, 64, 4, 1, 32, 2>;
+};
+template <typename T> using HeadFew = typename HeadFewOf<T>::S;
 
 struct HeadArgs {
     const bf16 *x, *w;           // [V][ld], [C][ld] as parts (stream_product.h)
@@ -509,16 +518,23 @@ template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a
 
 
 // workgroups of a launch: as many as are resident at once
-template <typename T> constexpr int head_resident() { return kCus * (int)(160 * 1024 / HeadShape<T>::kLds); }
-template <typename T> static unsigned head_grid(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, head_resident<T>()); }
+template <typename S> constexpr int head_resident() { return kCus * (int)(160 * 1024 / S::kLds); }
+template <typename T> static unsigned head_grid(int64_t tiles)
+{
+    return (unsigned)std::min<int64_t>(tiles, head_resident<HeadShape<T>>());
+}
 
 // ranges of class tiles: as many as fill the chip once
+template <typename S> static int ranges_of(int64_t V, int C)
+{
+    const int64_t tiles = ceil_div(C, S::BN), blocks = std::max<int64_t>(1, ceil_div(V, S::BM));
+    const int64_t ranges = std::min<int64_t>(tiles, std::max<int64_t>(1, head_resident<S>() / blocks));
+    return (int)ceil_div(tiles, ceil_div(tiles, ranges));
+}
+template <typename T> static bool head_few(int64_t V) { return V <= HeadFew<T>::BM; }
 template <typename T> static int head_ranges(int64_t V, int C)
 {
-    using S = HeadShape<T>;
-    const int64_t tiles = ceil_div(C, S::BN), blocks = std::max<int64_t>(1, ceil_div(V, S::BM));
-    const int64_t ranges = std::min<int64_t>(tiles, std::max<int64_t>(1, head_resident<T>() / blocks));
-    return (int)ceil_div(tiles, ceil_div(tiles, ranges));
+    return head_few<T>(V) ? ranges_of<HeadFew<T>>(V, C) : ranges_of<HeadShape<T>>(V, C);
 }
 
 // splits of a sum over K for an [M][N] result: the fewest (of at least 512 steps each, up to 32) that
@@ -526,7 +542,7 @@ template <typename T> static int head_ranges(int64_t V, int C)
 template <typename T> static int sum_splits(int64_t M, int64_t N, int64_t K)
 {
     using S = HeadShape<T>;
-    const int64_t tiles = ceil_div(M, S::BM) * ceil_div(N, S::BN), resident = head_resident<T>();
+    const int64_t tiles = ceil_div(M, S::BM) * ceil_div(N, S::BN), resident = head_resident<S>();
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(32, resident / tiles), K / 512));
     int64_t best = 1;
     double best_used = 0.0;
@@ -642,11 +658,18 @@ template <typename T, Layout QL, Sums SUMS> static int32_t launch_sum(const SumA
     return launch_status("linear_cross_entropy_bwd");
 }
 
+template <typename T, typename S>
+static void launch_stats(const HeadArgs &h, int ranges, float2 *stats, float *at_label, hipStream_t st)
+{
+    raise_lds<&head_stats<T, S>>(S::kLds);
+    hipLaunchKernelGGL((head_stats<T, S>), dim3((unsigned)(ceil_div(h.V, S::BM) * ranges)), dim3(S::kThreads), S::kLds, st, h,
+                       ranges, (int)ceil_div(ceil_div(h.C, S::BN), ranges), stats, at_label);
+}
+
 template <typename T>
 static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t reduction, float *loss, int32_t *count,
                             float *lse, void *ws, hipStream_t st)
 {
-    using S = HeadShape<T>;
     const HeadScratch<T> n(h.V, h.F, h.C, false);
     Carver carve(ws);
     bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w);
@@ -659,10 +682,8 @@ static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t re
     if (h.V > 0) {
         if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
         const int ranges = head_ranges<T>(h.V, h.C);
-        const int per_range = (int)ceil_div(ceil_div(h.C, S::BN), ranges);
-        raise_lds<&head_stats<T, S>>(S::kLds);
-        hipLaunchKernelGGL((head_stats<T, S>), dim3((unsigned)(ceil_div(h.V, S::BM) * ranges)), dim3(S::kThreads), S::kLds,
-                           st, h, ranges, per_range, stats, at_label);
+        if (head_few<T>(h.V)) launch_stats<T, HeadFew<T>>(h, ranges, stats, at_label, st);
+        else launch_stats<T, HeadShape<T>>(h, ranges, stats, at_label, st);
         int lanes = 1;      // four ranges a lane
         while (lanes < kWave && lanes * 4 < ranges) lanes *= 2;
         blocks = (int)ceil_div(h.V, kJoinThreads / lanes);

@@ -71,22 +71,27 @@ def nll_loss(log_probs, target):
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}      # JGAMD_LOSS_NONE, JGAMD_LOSS_MEAN, JGAMD_LOSS_SUM
 
 
-def _linear_forward(x, weight, bias, target, reduction):
-    """(loss, lse, count)"""
+def _linear_forward(x, weight, bias, target, reduction, for_backward):
+    """(loss, lse, count); without a backward pass the last two are not kept (one allocation less each)."""
     lib = _lib.load()
     dev = x.device
     V, F = x.shape
     C = weight.shape[0]
     code = _lib.dtype_code(x.dtype)
     loss = torch.empty((V,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-    count = torch.empty((), dtype=torch.int32, device=dev)
-    lse = torch.empty(V, dtype=torch.float32, device=dev)
     nbytes = _lib.query(lib.jgamd_linear_cross_entropy_workspace, V, F, C, code, 0)
-    ws = _lib.workspace(nbytes, dev)
+    if for_backward:
+        count = torch.empty((), dtype=torch.int32, device=dev)
+        lse = torch.empty(V, dtype=torch.float32, device=dev)
+        ws = _lib.workspace(nbytes, dev)
+        lse_at, count_at = _lib.ptr(lse), _lib.ptr(count)
+    else:
+        ws = _lib.workspace(nbytes + 4 * V + 4, dev)
+        lse, count, lse_at, count_at = None, None, ws.data_ptr() + nbytes, ws.data_ptr() + nbytes + 4 * V
     with _lib.on(dev):
         _lib.check(lib.jgamd_linear_cross_entropy_fwd(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(target),
                                                       1 if target.dtype == torch.int64 else 0, V, F, C, code, reduction,
-                                                      _lib.ptr(loss), _lib.ptr(count), _lib.ptr(lse), _lib.ptr(ws), nbytes,
+                                                      _lib.ptr(loss), count_at, lse_at, _lib.ptr(ws), nbytes,
                                                       _lib.stream_ptr(dev)))
     return loss, lse, count
 
@@ -94,7 +99,7 @@ def _linear_forward(x, weight, bias, target, reduction):
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, reduction):
-        loss, lse, count = _linear_forward(x, weight, bias, target, reduction)
+        loss, lse, count = _linear_forward(x, weight, bias, target, reduction, True)
         ctx.save_for_backward(x, weight, bias, target, lse, count)
         ctx.reduction = reduction
         return loss
@@ -158,5 +163,5 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
         bias = bias.contiguous()
     target = target.contiguous()
     if not _lib.needs_grad(x, weight, bias):
-        return _linear_forward(x, weight, bias, target, _REDUCTIONS[reduction])[0]
+        return _linear_forward(x, weight, bias, target, _REDUCTIONS[reduction], False)[0]
     return _LinearCrossEntropy.apply(x, weight, bias, target, _REDUCTIONS[reduction])
