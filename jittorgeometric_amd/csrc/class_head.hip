@@ -2,7 +2,8 @@
 // matrix of logits:
 //
 //     lse[i] = log sum_c exp(z[i,c]),   loss[i] = lse[i] - z[i,label[i]]     (0 without a label in [0,C))
-//     d[i,c] = g[i] (exp(z[i,c] - lse[i]) - [c == label[i]]),   dx = d w,   dw = d^T x,   db = sum_i d
+//     d[i,c] = exp(z[i,c] - lse[i]) - [c == label[i]]                        (0 without a label)
+//     dx[i] = g[i] d[i] w,   dw = d^T (g x),   db = sum_i g[i] d[i]
 //
 // Forward: a workgroup keeps BM rows and walks a range of class tiles.  A lane holds four
 // consecutive classes of one row, so the running maximum and sum of exponentials of a row are two
@@ -12,7 +13,10 @@
 // the classes (at most kPieceElements numbers, in the type of x); two products take it from there.
 // dx sums over the pieces and dw over the blocks of rows in fp32 (a workspace where several take
 // part), rounded once at the end.  Four products instead of the three of a loss that keeps its
-// logits.  d in bfloat16 is off by 2^-9 of itself, like any gradient of logits of that type.
+// logits.  d in bfloat16 is off by 2^-9 of itself, like any gradient of logits of that type; it is kept
+// without g, since -1 is exact but g (1 / rows) rounded once for all rows would shift every result alike
+// (16384 rows of 131072 classes: dw off by 3.1e-3 with g in d, 1.7e-3 without).  g multiplies the fp32
+// sums where it is one number, and dx's rows and a copy of x where it is one a row.
 //
 // Bound by the matrix units from some hundred rows on, by reading w below that.
 #include <algorithm>
@@ -111,11 +115,11 @@ __device__ __forceinline__ int tiles_of(int mtiles, int ntiles)
     return first < all ? (int)((all - 1 - first) / g + 1) : 0;
 }
 
-// Parts of an array: [R][F] of T to PARTS arrays [R][ld] of bfloat16, zero behind F.
-// grid: x = pieces of 8
+// Parts of an array: [R][F] of T to PARTS arrays [R][ld] of bfloat16, zero behind F; rows times scale[R]
+// unless that is NULL (a row times zero is zero whatever it holds).  grid: x = pieces of 8
 template <typename T>
-__global__ __launch_bounds__(256) void head_parts(const T *__restrict__ src, int64_t R, int F, int ld, bf16 *__restrict__ dst,
-                                                  int64_t part)
+__global__ __launch_bounds__(256) void head_parts(const T *__restrict__ src, const float *__restrict__ scale, int64_t R, int F,
+                                                  int ld, bf16 *__restrict__ dst, int64_t part)
 {
     const int across = ld / 8;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -125,6 +129,7 @@ __global__ __launch_bounds__(256) void head_parts(const T *__restrict__ src, int
     Eight<T> e;
     if (c + 8 <= F) e.load(src + row * F + c);
     else e.load_some(src + row * F + c, F - c);
+    if (scale) e.scale(scale[row]);
     e.store_parts(dst + row * ld + c, part);
 }
 
@@ -318,9 +323,7 @@ __global__ __launch_bounds__(kJoinThreads) void head_total(const double *__restr
 
 struct PieceArgs {
     HeadArgs head;             // of the whole problem
-    const float *lse, *grad;   // [V]; [1], or [V] with per_row
-    const int32_t *count;      // NULL: not a mean
-    int per_row;
+    const float *lse;          // [V]
     int64_t row0;              // the block of rows and the piece of classes
     int rows, c0, classes;
     bf16 *d;                   // [rows][ld] as parts
@@ -355,7 +358,6 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
     extern __shared__ __align__(16) char lds[];
     const int ntiles = (a.classes + S::BN - 1) / S::BN, mtiles = (a.rows + S::BM - 1) / S::BM;
     const HeadArgs &h = a.head;
-    const float all = a.per_row ? 0.f : a.grad[0] / (a.count ? (float)a.count[0] : 1.f);
     auto corner = [&](int t, int *m0, int *n0) {
         int m, n;
         bool exists;
@@ -390,7 +392,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
                 if (m >= a.rows) continue;
                 const int64_t row = a.row0 + m;
                 const int64_t label = head_label(h, row);
-                const float g = a.per_row ? a.grad[row] : all, l = a.lse[row];
+                const float l = a.lse[row];
                 const uint32_t keep = label < 0 ? 0u : 0xffffffffu;
                 const int at = label < 0 ? -1 : (int)(label - a.c0 - n0);
                 bf16 *out = a.d + m * (int64_t)a.ld + n0;
@@ -401,11 +403,11 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
                     // z - l is taken before the scaling: both may be large
 #pragma unroll
                     for (int r = 0; r < 8; r++)
-                        d[r] = g * __builtin_amdgcn_exp2f((acc[i + r / 4][j][r % 4] - l) * kLog2e);
+                        d[r] = __builtin_amdgcn_exp2f((acc[i + r / 4][j][r % 4] - l) * kLog2e);
                     if (at >= n && at < n + 8) {
 #pragma unroll
                         for (int r = 0; r < 8; r++)
-                            if (n + r == at) d[r] -= g;
+                            if (n + r == at) d[r] -= 1.f;
                     }
                     if (edge) {
                         if (n0 + n >= a.ld) continue;
@@ -419,8 +421,8 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
         });
 }
 
-// out[m][n] = (first ? 0 : acc[m][n]) + sum_k P[n][k] Q[m][k], to `out` when `last`, else to `acc`; with
-// several splits of k every split leaves its sum in part and head_join finishes.
+// out[m][n] = g ((first ? 0 : acc[m][n]) + sum_k P[n][k] Q[m][k]) when `last`, else the sum alone to
+// `acc`; with several splits of k every split leaves its sum in part and head_join finishes.
 struct SumArgs {
     const bf16 *p, *q;
     int64_t part_p, part_q;
@@ -430,11 +432,23 @@ struct SumArgs {
     float *acc, *part;  // [M][N], [splits][M][N]
     void *out_b;        // sums of Q over k, [M]; the same three arrays for them, NULL: not wanted
     float *acc_b, *part_b;
+    const float *row_scale;      // g of m, or NULL:
+    const float *grad;           // g = grad[0] (/ count[0]); both NULL: 1
+    const int32_t *count;
     int first, last;
     int whole;          // four neighbouring values lie on an address that one access can take
 };
 
-template <typename T> __device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc, int64_t at, f32x4 v, int n)
+__device__ __forceinline__ float sum_scale(const SumArgs &a, int m)
+{
+    if (a.row_scale) return a.row_scale[m];
+    if (!a.grad) return 1.f;
+    if (!a.count) return a.grad[0];
+    return a.count[0] > 0 ? a.grad[0] / (float)a.count[0] : 0.f;      // no row counts: every sum is zero
+}
+
+template <typename T>
+__device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc, int64_t at, f32x4 v, int n, float g)
 {
     if (!a.first) {
         if (a.whole && n >= 4) v += *reinterpret_cast<const f32x4 *>(acc + at);
@@ -444,7 +458,7 @@ template <typename T> __device__ __forceinline__ void finish4(const SumArgs &a, 
                 if (r < n) v[r] += acc[at + r];
         }
     }
-    if (a.last) store4<T>(static_cast<T *>(out) + at, v, n, a.whole);
+    if (a.last) store4<T>(static_cast<T *>(out) + at, v * g, n, a.whole);
     else store4<float>(acc + at, v, n, a.whole);
 }
 
@@ -481,9 +495,10 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
             for (int j = 0; j < S::FM; j++) {
                 const int m = m0 + Product::m_of(j);
                 if (m >= a.M) continue;
+                const float g = a.splits > 1 ? 1.f : sum_scale(a, m);
                 if (SUMS == kSumQ && n0 == 0 && Product::n_of(0) == 0) {
                     if (a.splits > 1) a.part_b[(int64_t)split * a.M + m] = sums[j][0];
-                    else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1);
+                    else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1, g);
                 }
 #pragma unroll
                 for (int i = 0; i < S::FN; i++) {
@@ -491,7 +506,7 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
                     if (n >= a.N) continue;
                     const int64_t at = (int64_t)m * a.N + n;
                     if (a.splits > 1) store4<float>(a.part + (int64_t)split * a.M * a.N + at, acc[i][j], a.N - n, a.whole);
-                    else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n);
+                    else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n, g);
                 }
             }
         });
@@ -511,11 +526,55 @@ template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a
         float *acc = b ? a.acc_b : a.acc;
         float v = a.first ? 0.f : acc[at];
         for (int k = 0; k < a.splits; k++) v += part[k * stride + at];
-        if (a.last) static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v);
+        if (a.last) static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v * sum_scale(a, b ? (int)at : (int)(at / a.N)));
         else acc[at] = v;
     }
 }
 
+
+// g of every row: grad where the row has a label, else zero.  grid: x = rows / 256
+__global__ __launch_bounds__(256) void head_row_scale(HeadArgs a, const float *__restrict__ grad, float *__restrict__ scale)
+{
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row < a.V) scale[row] = head_label(a, row) >= 0 ? grad[row] : 0.f;
+}
+
+// db of a piece with one g a row: acc[c] (+)= sum_m scale[m] d[m][c] over the block's rows, rounded to out
+// when `last`.  A workgroup has 64 classes, 32 strands of rows.  grid: x = classes / 64
+template <typename T>
+__global__ __launch_bounds__(256) void head_bias(const bf16 *__restrict__ d, int64_t part, int ld, int rows, int classes,
+                                                 const float *__restrict__ scale, float *__restrict__ acc, T *__restrict__ out,
+                                                 int first, int last)
+{
+    __shared__ float strands[32][65];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 7) * 8, strand = threadIdx.x >> 3;
+    float v[8] = {};
+    if (c < classes) {      // ld is a multiple of 8 and holds zeros behind the last class
+#pragma unroll 4
+        for (int m = strand; m < rows; m += 32) {
+            const float g = scale[m];
+#pragma unroll
+            for (int s = 0; s < HeadShape<T>::kParts; s++) {
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(d + s * part + (int64_t)m * ld + c);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v[2 * i] = fmaf(g, bf16_lo(w[i]), v[2 * i]);
+                    v[2 * i + 1] = fmaf(g, bf16_hi(w[i]), v[2 * i + 1]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) strands[strand][(threadIdx.x & 7) * 8 + i] = v[i];
+    __syncthreads();
+    const int n = blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && n < classes) {
+        float sum = first ? 0.f : acc[n];
+        for (int k = 0; k < 32; k++) sum += strands[k][threadIdx.x];
+        if (last) out[n] = from_float<T>(sum);
+        else acc[n] = sum;
+    }
+}
 
 // workgroups of a launch: as many as are resident at once
 template <typename S> constexpr int head_resident() { return kCus * (int)(160 * 1024 / S::kLds); }
@@ -579,7 +638,8 @@ template <typename T> static size_t parts_elements(int64_t R, int F)
 }
 
 template <typename T> struct HeadScratch {      // of the forward pass, then of the backward pass
-    size_t x = 0, w = 0;                                              // bfloat16
+    size_t x = 0, w = 0, gx = 0;                                      // bfloat16
+    size_t scale = 0;                                                 // float
     size_t stats = 0, at_label = 0, blocks = 0;                       // float2, float, double + int
     size_t d = 0;                                                     // bfloat16
     size_t part = 0, part_b = 0, acc_x = 0, acc_w = 0, acc_b = 0;     // float
@@ -594,6 +654,8 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
             return;
         }
         const Pieces s = head_pieces<T>(V, C);
+        gx = (size_t)(V * parts_ld(F) * HeadShape<T>::kParts);
+        scale = (size_t)V;
         d = (size_t)(s.rows * (s.classes + kPad) * HeadShape<T>::kParts);
         const int64_t sx = sum_splits<T>(s.rows, F, s.classes), sw = sum_splits<T>(s.classes, F, s.rows);
         part = (size_t)std::max(sx > 1 ? sx * s.rows * F : 0, sw > 1 ? sw * s.classes * F : 0);
@@ -604,7 +666,7 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
     }
     size_t bytes() const
     {
-        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
+        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(gx, 2) + carve_bytes(scale, 4) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
                carve_bytes(blocks, 8) + carve_bytes(blocks, 4) + carve_bytes(d, 2) + carve_bytes(part, 4) +
                carve_bytes(part_b, 4) + carve_bytes(acc_x, 4) + carve_bytes(acc_w, 4) + carve_bytes(acc_b, 4);
     }
@@ -620,6 +682,15 @@ static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int3
     if (reduction < 0 || reduction > JGAMD_LOSS_SUM) return fail(JGAMD_ERR_SIZE, "%s: unknown reduction %d", who, reduction);
     return 0;
 }
+template <typename T>
+static void head_copy(const void *src, const float *scale, int64_t R, const HeadArgs &h, bf16 *dst, int64_t part, hipStream_t s)
+{
+    const int64_t pieces = R * (h.ld / 8);
+    if (pieces > 0)
+        hipLaunchKernelGGL((head_parts<T>), dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, s,
+                           static_cast<const T *>(src), scale, R, h.F, h.ld, dst, part);
+}
+
 // x and w as parts: copies into the workspace, or the arrays themselves
 template <typename T>
 static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs, bf16 *ws, hipStream_t s)
@@ -634,14 +705,8 @@ static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs
     }
     h->x = xs;
     h->w = ws;
-    auto copy = [&](const void *src, int64_t R, bf16 *dst, int64_t part) {
-        const int64_t pieces = R * (h->ld / 8);
-        if (pieces > 0)
-            hipLaunchKernelGGL((head_parts<T>), dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, s,
-                               static_cast<const T *>(src), R, h->F, h->ld, dst, part);
-    };
-    copy(x, h->V, xs, h->part_x);
-    copy(w, h->C, ws, h->part_w);
+    head_copy<T>(x, nullptr, h->V, *h, xs, h->part_x, s);
+    head_copy<T>(w, nullptr, h->C, *h, ws, h->part_w, s);
     return launch_status("linear_cross_entropy");
 }
 
@@ -703,12 +768,19 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
     const Pieces s = head_pieces<T>(h.V, h.C);
     const HeadScratch<T> n(h.V, h.F, h.C, true);
     Carver carve(ws);
-    bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w), *d = carve.take<bf16>(n.d);
+    bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w), *gx = carve.take<bf16>(n.gx);
+    float *scale = carve.take<float>(n.scale);
+    bf16 *d = carve.take<bf16>(n.d);
     float *part = carve.take<float>(n.part), *part_b = carve.take<float>(n.part_b);
     float *acc_x = carve.take<float>(n.acc_x), *acc_w = carve.take<float>(n.acc_w), *acc_b = carve.take<float>(n.acc_b);
     if (h.V > 0)
         if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
     if (h.V == 0) h.ld = (int)parts_ld(h.F);
+    const bool per_row = reduction == JGAMD_LOSS_NONE;
+    if (per_row && h.V > 0) {
+        hipLaunchKernelGGL(head_row_scale, dim3((unsigned)ceil_div(h.V, 256)), dim3(256), 0, st, h, grad, scale);
+        if (dw) head_copy<T>(x, scale, h.V, h, gx, h.V * h.ld, st);
+    }
     const int ldd = (int)s.classes + kPad;
     const int64_t part_d = s.rows * ldd;
     auto whole = [](int N, const void *p) { return N % 4 == 0 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0; };
@@ -718,8 +790,7 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
         for (int64_t c = 0; c < s.pieces; c++) {
             const int c0 = (int)(c * s.classes), classes = (int)std::min<int64_t>(s.classes, h.C - c0);
             if (rows > 0) {
-                const PieceArgs a{h, lse, grad, reduction == JGAMD_LOSS_MEAN ? count : nullptr,
-                                  reduction == JGAMD_LOSS_NONE, row0, rows, c0, classes, d, part_d, ldd};
+                const PieceArgs a{h, lse, row0, rows, c0, classes, d, part_d, ldd};
                 raise_lds<&head_piece<T, S>>(S::kLds);
                 hipLaunchKernelGGL((head_piece<T, S>), dim3(head_grid<T>(ceil_div(classes, S::BN) * ceil_div(rows, S::BM))),
                                    dim3(S::kThreads), S::kLds, st, a);
@@ -727,7 +798,9 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
             }
             SumArgs a{};
             a.q = d, a.part_q = part_d, a.ldq = ldd, a.ldp = h.ld, a.N = h.F, a.part = part;
+            a.grad = per_row ? nullptr : grad, a.count = reduction == JGAMD_LOSS_MEAN ? count : nullptr;
             if (dx && rows > 0) {
+                a.row_scale = per_row ? scale + row0 : nullptr;
                 a.p = h.w + (int64_t)c0 * h.ld, a.part_p = h.part_w;
                 a.M = rows, a.K = classes;
                 a.splits = sum_splits<T>(s.rows, h.F, s.classes);
@@ -737,14 +810,19 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
                 if (int32_t rc = launch_sum<T, kAlongK, kNoSums>(a, st)) return rc;
             }
             if (dw) {
-                a.p = h.x + row0 * h.ld, a.part_p = h.part_x;
+                a.p = (per_row ? gx : h.x) + row0 * h.ld, a.part_p = per_row ? h.V * h.ld : h.part_x;
+                a.row_scale = nullptr;
                 a.M = classes, a.K = rows;
                 a.splits = sum_splits<T>(s.classes, h.F, s.rows);
                 a.k_split = (int)(ceil_div(ceil_div(s.rows, a.splits), 64) * 64);
                 a.out = dw + (int64_t)c0 * h.F, a.acc = s.blocks > 1 ? acc_w + (int64_t)c0 * h.F : nullptr;
-                a.out_b = db ? db + c0 : nullptr, a.acc_b = s.blocks > 1 ? acc_b + c0 : nullptr, a.part_b = part_b;
+                const bool sums = db && !per_row;      // db beside dw
+                a.out_b = sums ? db + c0 : nullptr, a.acc_b = s.blocks > 1 ? acc_b + c0 : nullptr, a.part_b = part_b;
                 a.first = b == 0, a.last = b == s.blocks - 1, a.whole = whole(h.F, a.out);
-                const int32_t rc = db ? launch_sum<T, kAcrossK, kSumQ>(a, st) : launch_sum<T, kAcrossK, kNoSums>(a, st);
+                if (db && per_row)
+                    hipLaunchKernelGGL((head_bias<T>), dim3((unsigned)ceil_div(classes, 64)), dim3(256), 0, st, d, part_d, ldd,
+                                       rows, classes, scale + row0, a.acc_b, db + c0, a.first, a.last);
+                const int32_t rc = sums ? launch_sum<T, kAcrossK, kSumQ>(a, st) : launch_sum<T, kAcrossK, kNoSums>(a, st);
                 if (rc) return rc;
             }
         }

@@ -72,6 +72,11 @@ template <> struct Eight<bf16> {
     __device__ __forceinline__ void clear() { v = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void store(char *lds, int) const { *reinterpret_cast<u32x4 *>(lds) = v; }
     __device__ __forceinline__ void store_parts(bf16 *out, int64_t) const { *reinterpret_cast<u32x4 *>(out) = v; }
+    __device__ __forceinline__ void scale(float g)      // zero makes zero of anything
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = g == 0.f ? 0u : pack_bf16(g * bf16_lo(v[i]), g * bf16_hi(v[i]));
+    }
 };
 template <> struct Eight<float> {
     f32x4 a, b;
@@ -97,6 +102,11 @@ template <> struct Eight<float> {
     __device__ __forceinline__ void store_parts(bf16 *out, int64_t part) const
     {
         split([&](int s, u32x4 w) { *reinterpret_cast<u32x4 *>(out + s * part) = w; });
+    }
+    __device__ __forceinline__ void scale(float g)
+    {
+        if (g == 0.f) clear();
+        else a *= g, b *= g;
     }
     template <typename Put> __device__ __forceinline__ void split(Put &&put) const
     {
