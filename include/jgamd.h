@@ -400,7 +400,7 @@ int32_t jgamd_dense_rows(const float *x1, const float *w1, int32_t K1, const flo
  * NULL; db needs dw) from grad ([1], or [V] with JGAMD_LOSS_NONE) and the
  * forward's lse and count.  The workspace (the query with backward = 1) holds
  * the gradient of the logits for a block of rows and a piece of the classes
- * (at most 512 MB), and fp32 sums.  Fixed order, no atomics.  bfloat16 x and w
+ * (at most 1 GB), and fp32 sums.  Fixed order, no atomics.  bfloat16 x and w
  * with F a multiple of 8 must lie on 16-byte addresses; fp32, and other widths,
  * are laid out anew in the workspace.
  * With few classes: jgamd_cross_entropy_fwd / _bwd on logits

@@ -10,7 +10,7 @@
 // registers of a lane; lanes, wavefronts and ranges are joined at the end, in a fixed order.
 //
 // Backward: z is computed again, tile by tile, and d is written for a block of rows and a piece of
-// the classes (at most kPieceElements numbers, in the type of x); two products take it from there.
+// the classes (at most kPieceBytes, in the type of x); two products take it from there.
 // dx sums over the pieces and dw over the blocks of rows in fp32 (a workspace where several take
 // part), rounded once at the end.  Four products instead of the three of a loss that keeps its
 // logits.  d in bfloat16 is off by 2^-9 of itself, like any gradient of logits of that type; it is kept
@@ -27,21 +27,22 @@
 namespace jg {
 
 constexpr int kHeadMaxFeatures = 1 << 20;
-constexpr int64_t kPieceElements = (int64_t)1 << 28;
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;      // of d.  16384 rows, 512 features, 131072 classes, bfloat16: 9.7 ms with pieces of 512 MB, 9.4 with 1 GB
 constexpr int kBlockRows = 16384;      // rows of a block of the backward pass
 constexpr int kJoinThreads = 256;
 constexpr int kCus = 256;
+constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kPad = 128;      // classes between the rows of d: rows a power of two apart meet in one channel of the L2
 
 // bfloat16: 256 x 128 results, four wavefronts of 128 x 64, three stages (72 KB of LDS): two workgroups
 // a compute unit, one of which multiplies while the other writes its results.
-// float: three parts an operand, 256 x 128 results, two stages (144 KB).
+// float: the same tile of two parts an operand, steps of 32 (128 KB).
 template <typename T> struct HeadShapeOf;
 template <> struct HeadShapeOf<bf16> {
     using S = StreamShape<1, 256, 256, 2, 4, 64, 2>;
 };
 template <> struct HeadShapeOf<float> {
-    using S = StreamShape<3, 256, 128, 4, 2, 32, 2>;
+    using S = StreamShape<2, 256, 256, 2, 4, 32, 2>;
 };
 template <typename T> using HeadShape = typename HeadShapeOf<T>::S;
 // the forward pass of a few rows: all of w streams past one tile of them, two workgroups a compute unit
@@ -50,12 +51,21 @@ template <> struct HeadFewOf<bf16> {
     using S = StreamShape<1, 128, 32, 4, 1, 64, 4>;
 };
 template <> struct HeadFewOf<float> {
-    using S = StreamShape<3, 128, 64, 4, 1, 32, 2>;
+    using S = StreamShape<2, 128, 64, 4, 1, 32, 3>;
 };
 template <typename T> using HeadFew = typename HeadFewOf<T>::S;
 
+// Floats enter as two float16 parts: a 2^e = a1 + a2, each the remainder rounded to 11 bits, which is
+// all of a's 24 bits but the last; e brings the array's largest entry to 2^14 .. 2^15.  Dropping a2 b2
+// (under 2^-24 of a b) leaves three products, half of what three bfloat16 parts take.  float16 ends at
+// 2^-24: an entry under 2^-17 of the array's largest keeps an absolute precision of 2^-39 of that largest
+// instead of 24 bits of its own.  d is stored times 2^15 (|d| <= 1): probabilities under 2^-17 keep 2^-40.
+constexpr int kDExponent = 15;
+constexpr int kMaxBlocks = 256;      // workgroups that look for an array's largest entry
+
 struct HeadArgs {
     const bf16 *x, *w;           // [V][ld], [C][ld] as parts (stream_product.h)
+    const int *exponents;        // e of x, w, g x where they are split, else NULL
     int64_t part_x, part_w;
     int ld;                      // F rounded up to 8
     const void *bias;            // [C] of T, or NULL
@@ -70,6 +80,9 @@ __device__ __forceinline__ int64_t head_label(const HeadArgs &a, int64_t row)
     const int64_t y = a.y64 ? a.y64[row] : (int64_t)a.y32[row];
     return y >= 0 && y < a.C ? y : -1;
 }
+
+// 2^-(e1 + e2), as near as a float comes
+__device__ __forceinline__ float unscale(int e1, int e2) { return ldexpf(1.f, min(max(-(e1 + e2), -126), 127)); }
 
 // (m, s): s exponentials relative to m.  An m of -inf holds nothing (s = 0).
 __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s2)
@@ -115,22 +128,136 @@ __device__ __forceinline__ int tiles_of(int mtiles, int ntiles)
     return first < all ? (int)((all - 1 - first) / g + 1) : 0;
 }
 
-// Parts of an array: [R][F] of T to PARTS arrays [R][ld] of bfloat16, zero behind F; rows times scale[R]
-// unless that is NULL (a row times zero is zero whatever it holds).  grid: x = pieces of 8
-template <typename T>
-__global__ __launch_bounds__(256) void head_parts(const T *__restrict__ src, const float *__restrict__ scale, int64_t R, int F,
-                                                  int ld, bf16 *__restrict__ dst, int64_t part)
+// two floats as two float16 in one register, rounded to nearest even
+__device__ __forceinline__ uint32_t pack_half(float a, float b)
+{
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 v = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ float half_lo(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)v); }
+__device__ __forceinline__ float half_hi(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16)); }
+
+// eight neighbouring values as one bfloat16 or two float16 parts, kept where `keep` has ones
+template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int64_t part, float (&v)[8], uint32_t keep)
+{
+#pragma unroll
+    for (int s = 0; s < PARTS; s++) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            w[i] = PARTS == 1 ? pack_bf16(v[2 * i], v[2 * i + 1]) : pack_half(v[2 * i], v[2 * i + 1]);
+            if (s + 1 < PARTS) {
+                v[2 * i] -= half_lo(w[i]);
+                v[2 * i + 1] -= half_hi(w[i]);
+            }
+            w[i] &= keep;
+        }
+        *reinterpret_cast<u32x4 *>(out + s * part) = w;
+    }
+}
+
+// One array to be laid out as parts: [R][F] of T to [R][ld], zero behind F; rows times scale[R] unless
+// that is NULL (a row times zero is zero whatever it holds).
+struct Copy {
+    const void *src;
+    const float *scale;
+    int64_t R;
+    bf16 *dst;
+    int64_t part;            // elements between the parts
+    uint32_t *largest;       // [kMaxBlocks]: bits of the largest finite |entry| each workgroup saw
+    int *exponent;
+};
+struct Copies {
+    Copy of[2];
+    int blocks0;             // workgroups of the first; the others have the second
+    int F, ld;
+};
+
+// piece `id` of 8 entries of an array
+template <typename T> __device__ __forceinline__ Eight<T> copy_piece(const Copy &c, int F, int ld, int64_t id)
 {
     const int across = ld / 8;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= R * across) return;
     const int64_t row = id / across;
-    const int c = (int)(id - row * across) * 8;
+    const int at = (int)(id - row * across) * 8;
     Eight<T> e;
-    if (c + 8 <= F) e.load(src + row * F + c);
-    else e.load_some(src + row * F + c, F - c);
-    if (scale) e.scale(scale[row]);
-    e.store_parts(dst + row * ld + c, part);
+    const T *src = static_cast<const T *>(c.src) + row * F + at;
+    if (at + 8 <= F) e.load(src);
+    else e.load_some(src, F - at);
+    if (c.scale) e.scale(c.scale[row]);
+    return e;
+}
+
+// grid: x = kMaxBlocks for each of the arrays
+__global__ __launch_bounds__(256) void head_largest(Copies a)
+{
+    __shared__ uint32_t s_top[4];
+    const Copy &c = a.of[blockIdx.x >= (unsigned)kMaxBlocks];
+    const int block = blockIdx.x % kMaxBlocks;
+    const int64_t pieces = c.R * (a.ld / 8);
+    uint32_t top = 0;
+    auto see = [&](float v) {
+        const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
+        top = max(top, bits < 0x7f800000u ? bits : 0u);
+    };
+#pragma unroll 4
+    for (int64_t id = (int64_t)block * 256 + threadIdx.x; id < pieces; id += kMaxBlocks * 256) {
+        const Eight<float> e = copy_piece<float>(c, a.F, a.ld, id);
+#pragma unroll
+        for (int i = 0; i < 4; i++) see(e.a[i]), see(e.b[i]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
+    if (lane_id() == 0) s_top[wave_in_block()] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) c.largest[block] = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+}
+
+// grid: x = blocks0 + the second array's, 256 pieces of 8 each
+template <typename T> __global__ __launch_bounds__(256) void head_parts(Copies a)
+{
+    const bool second = (int)blockIdx.x >= a.blocks0;
+    const Copy &c = a.of[second];
+    const int block = second ? blockIdx.x - a.blocks0 : blockIdx.x;
+    float up = 1.f;
+    if constexpr (sizeof(T) == 4) {      // the exponent, by every workgroup for itself
+        static_assert(kMaxBlocks == 256, "a thread looks at one");
+        __shared__ uint32_t s_top[4];
+        uint32_t top = c.largest[threadIdx.x];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
+        if (lane_id() == 0) s_top[wave_in_block()] = top;
+        __syncthreads();
+        top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+        const int e = top == 0 ? 0 : min(14 - ((int)(top >> 23) - 127), 126);      // a subnormal counts as 2^-127
+        up = ldexpf(1.f, e);
+        if (block == 0 && threadIdx.x == 0) *c.exponent = e;
+    }
+    const int64_t id = (int64_t)block * 256 + threadIdx.x;
+    if (id >= c.R * (a.ld / 8)) return;
+    const Eight<T> e = copy_piece<T>(c, a.F, a.ld, id);
+    if constexpr (sizeof(T) == 4) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = e.a[i] * up, v[4 + i] = e.b[i] * up;
+        store_parts8<2>(c.dst + id * 8, c.part, v, 0xffffffffu);
+    } else *reinterpret_cast<u32x4 *>(c.dst + id * 8) = e.v;
+}
+
+// a tile's sums, of classes c0 and up, to logits
+template <typename T, typename Product, typename S>
+__device__ __forceinline__ void logits(f32x4 (&acc)[S::FN][S::FM], const HeadArgs &h, int c0)
+{
+    if (S::kParts == 1 && !h.bias) return;
+    const float down = S::kParts == 2 ? unscale(h.exponents[0], h.exponents[1]) : 1.f;
+#pragma unroll
+    for (int i = 0; i < S::FN; i++) {
+        const f32x4 b = bias4<T>(h.bias, c0 + Product::n_of(i), h.C);
+#pragma unroll
+        for (int j = 0; j < S::FM; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[i][j][r] = S::kParts == 2 ? fmaf(acc[i][j][r], down, b[r]) : acc[i][j][r] + b[r];
+    }
 }
 
 // grid: x = blocks of BM rows x ranges of class tiles.  stats [ranges][V]
@@ -166,14 +293,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void head_stats(HeadArgs a, int ran
         },
         [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *) {
             const int c0 = (first + t) * S::BN;
-            if (a.bias) {
-#pragma unroll
-                for (int i = 0; i < S::FN; i++) {
-                    const f32x4 b = bias4<T>(a.bias, c0 + Product::n_of(i), a.C);
-#pragma unroll
-                    for (int j = 0; j < S::FM; j++) acc[i][j] += b;
-                }
-            }
+            logits<T, Product, S>(acc, a, c0);
             if (c0 + S::BN > a.C) {      // classes past the last count as -inf
 #pragma unroll
                 for (int i = 0; i < S::FN; i++)
@@ -189,13 +309,13 @@ __global__ __launch_bounds__(S::kThreads, 2) void head_stats(HeadArgs a, int ran
 #pragma unroll
                 for (int i = 0; i < S::FN; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) top = fmaxf(top, acc[i][j][r]);
+                    for (int r = 0; r < 4; r += 2) top = fmaxf(fmaxf(top, acc[i][j][r]), acc[i][j][r + 1]);
                 const float ref = top == -INFINITY ? 0.f : top;
                 float sum = s[j] * __expf(m[j] - ref);
 #pragma unroll
                 for (int i = 0; i < S::FN; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) sum += __expf(acc[i][j][r] - ref);
+                    for (int r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
                 m[j] = top;
                 s[j] = sum;
                 // the one lane that holds the label's logit hands it on
@@ -331,25 +451,6 @@ struct PieceArgs {
     int ld;
 };
 
-// eight neighbouring values as parts, kept where `keep` has ones
-template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int64_t part, float (&v)[8], uint32_t keep)
-{
-#pragma unroll
-    for (int s = 0; s < PARTS; s++) {
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-            if (s + 1 < PARTS) {
-                v[2 * i] -= bf16_lo(w[i]);
-                v[2 * i + 1] -= bf16_hi(w[i]);
-            }
-            w[i] &= keep;
-        }
-        *reinterpret_cast<u32x4 *>(out + s * part) = w;
-    }
-}
-
 // d for a block of rows and a piece of classes.  Classes between the last and ld are written as zero.
 // grid: x = workgroups, each with every gridDim.x-th tile
 template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) void head_piece(PieceArgs a)
@@ -376,15 +477,8 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
         [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *) {
             int m0, n0;
             corner(t, &m0, &n0);
-            if (h.bias) {
-#pragma unroll
-                for (int i = 0; i < S::FN; i++) {
-                    const f32x4 b = bias4<T>(h.bias, a.c0 + n0 + Product::n_of(i), h.C);
-#pragma unroll
-                    for (int j = 0; j < S::FM; j++) acc[i][j] += b;
-                }
-            }
-            constexpr float kLog2e = 1.44269504088896341f;
+            logits<T, Product, S>(acc, h, a.c0 + n0);
+            constexpr float kUp = S::kParts == 2 ? kDExponent : 0, kOne = S::kParts == 2 ? 1 << kDExponent : 1;
             const bool edge = n0 + S::BN > a.classes;
 #pragma unroll
             for (int j = 0; j < S::FM; j++) {
@@ -403,11 +497,11 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
                     // z - l is taken before the scaling: both may be large
 #pragma unroll
                     for (int r = 0; r < 8; r++)
-                        d[r] = __builtin_amdgcn_exp2f((acc[i + r / 4][j][r % 4] - l) * kLog2e);
+                        d[r] = __builtin_amdgcn_exp2f(fmaf(acc[i + r / 4][j][r % 4] - l, kLog2e, kUp));
                     if (at >= n && at < n + 8) {
 #pragma unroll
                         for (int r = 0; r < 8; r++)
-                            if (n + r == at) d[r] -= 1.f;
+                            if (n + r == at) d[r] -= kOne;
                     }
                     if (edge) {
                         if (n0 + n >= a.ld) continue;
@@ -432,6 +526,7 @@ struct SumArgs {
     float *acc, *part;  // [M][N], [splits][M][N]
     void *out_b;        // sums of Q over k, [M]; the same three arrays for them, NULL: not wanted
     float *acc_b, *part_b;
+    const int *exponent_p;       // e of P where the operands are split (those of Q: kDExponent), else NULL
     const float *row_scale;      // g of m, or NULL:
     const float *grad;           // g = grad[0] (/ count[0]); both NULL: 1
     const int32_t *count;
@@ -439,12 +534,13 @@ struct SumArgs {
     int whole;          // four neighbouring values lie on an address that one access can take
 };
 
-__device__ __forceinline__ float sum_scale(const SumArgs &a, int m)
+__device__ __forceinline__ float sum_scale(const SumArgs &a, int m, bool sum_of_q)
 {
-    if (a.row_scale) return a.row_scale[m];
-    if (!a.grad) return 1.f;
-    if (!a.count) return a.grad[0];
-    return a.count[0] > 0 ? a.grad[0] / (float)a.count[0] : 0.f;      // no row counts: every sum is zero
+    const float down = a.exponent_p ? unscale(kDExponent, sum_of_q ? 0 : *a.exponent_p) : 1.f;
+    if (a.row_scale) return down * a.row_scale[m];
+    if (!a.grad) return down;
+    if (!a.count) return down * a.grad[0];
+    return a.count[0] > 0 ? down * (a.grad[0] / (float)a.count[0]) : 0.f;      // no row counts: every sum is zero
 }
 
 template <typename T>
@@ -495,10 +591,10 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
             for (int j = 0; j < S::FM; j++) {
                 const int m = m0 + Product::m_of(j);
                 if (m >= a.M) continue;
-                const float g = a.splits > 1 ? 1.f : sum_scale(a, m);
+                const float g = a.splits > 1 ? 1.f : sum_scale(a, m, false);
                 if (SUMS == kSumQ && n0 == 0 && Product::n_of(0) == 0) {
                     if (a.splits > 1) a.part_b[(int64_t)split * a.M + m] = sums[j][0];
-                    else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1, g);
+                    else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1, sum_scale(a, m, true));
                 }
 #pragma unroll
                 for (int i = 0; i < S::FN; i++) {
@@ -516,6 +612,7 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
 template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a)
 {
     const int64_t size = (int64_t)a.M * a.N, all = size + (a.out_b ? a.M : 0);
+    const float g = a.last && !a.row_scale ? sum_scale(a, 0, false) : 1.f, g_b = a.last && a.out_b ? sum_scale(a, 0, true) : 1.f;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
         const int64_t e = (int64_t)blockIdx.x * 1024 + u * 256 + threadIdx.x;
@@ -526,7 +623,7 @@ template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a
         float *acc = b ? a.acc_b : a.acc;
         float v = a.first ? 0.f : acc[at];
         for (int k = 0; k < a.splits; k++) v += part[k * stride + at];
-        if (a.last) static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v * sum_scale(a, b ? (int)at : (int)(at / a.N)));
+        if (a.last) static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v * (b ? g_b : a.row_scale ? sum_scale(a, (int)(at / a.N), false) : g));
         else acc[at] = v;
     }
 }
@@ -552,14 +649,14 @@ __global__ __launch_bounds__(256) void head_bias(const bf16 *__restrict__ d, int
     if (c < classes) {      // ld is a multiple of 8 and holds zeros behind the last class
 #pragma unroll 4
         for (int m = strand; m < rows; m += 32) {
-            const float g = scale[m];
+            const float g = sizeof(T) == 2 ? scale[m] : scale[m] / (1 << kDExponent);
 #pragma unroll
             for (int s = 0; s < HeadShape<T>::kParts; s++) {
                 const u32x4 w = *reinterpret_cast<const u32x4 *>(d + s * part + (int64_t)m * ld + c);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    v[2 * i] = fmaf(g, bf16_lo(w[i]), v[2 * i]);
-                    v[2 * i + 1] = fmaf(g, bf16_hi(w[i]), v[2 * i + 1]);
+                    v[2 * i] = fmaf(g, sizeof(T) == 2 ? bf16_lo(w[i]) : half_lo(w[i]), v[2 * i]);
+                    v[2 * i + 1] = fmaf(g, sizeof(T) == 2 ? bf16_hi(w[i]) : half_hi(w[i]), v[2 * i + 1]);
                 }
             }
         }
@@ -623,7 +720,7 @@ template <typename T> static Pieces head_pieces(int64_t V, int C)
     Pieces s;
     s.rows = std::min<int64_t>(std::max<int64_t>(V, 1), kBlockRows);
     s.blocks = std::max<int64_t>(1, ceil_div(V, s.rows));
-    s.classes = std::max<int64_t>(tile, kPieceElements / s.rows / tile * tile);
+    s.classes = std::max<int64_t>(tile, kPieceBytes / (2 * HeadShape<T>::kParts) / s.rows / tile * tile);
     s.classes = std::min<int64_t>(s.classes, ceil_div(C, 8) * 8);
     s.pieces = ceil_div(C, s.classes);
     return s;
@@ -639,7 +736,7 @@ template <typename T> static size_t parts_elements(int64_t R, int F)
 
 template <typename T> struct HeadScratch {      // of the forward pass, then of the backward pass
     size_t x = 0, w = 0, gx = 0;                                      // bfloat16
-    size_t scale = 0;                                                 // float
+    size_t largest = 0, scale = 0;                                    // uint32_t (and the exponents), float
     size_t stats = 0, at_label = 0, blocks = 0;                       // float2, float, double + int
     size_t d = 0;                                                     // bfloat16
     size_t part = 0, part_b = 0, acc_x = 0, acc_w = 0, acc_b = 0;     // float
@@ -647,6 +744,7 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
     {
         x = parts_elements<T>(V, F);
         w = parts_elements<T>(C, F);
+        largest = sizeof(T) == 4 ? 3 * kMaxBlocks + 3 : 0;
         if (!backward) {
             stats = (size_t)head_ranges<T>(V, C) * V;
             at_label = (size_t)V;
@@ -666,7 +764,8 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
     }
     size_t bytes() const
     {
-        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(gx, 2) + carve_bytes(scale, 4) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
+        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(gx, 2) + carve_bytes(largest, 4) +
+               carve_bytes(scale, 4) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
                carve_bytes(blocks, 8) + carve_bytes(blocks, 4) + carve_bytes(d, 2) + carve_bytes(part, 4) +
                carve_bytes(part_b, 4) + carve_bytes(acc_x, 4) + carve_bytes(acc_w, 4) + carve_bytes(acc_b, 4);
     }
@@ -682,22 +781,31 @@ static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int3
     if (reduction < 0 || reduction > JGAMD_LOSS_SUM) return fail(JGAMD_ERR_SIZE, "%s: unknown reduction %d", who, reduction);
     return 0;
 }
+// lays out one or two arrays as parts; `numbers`: the first one's place among the three that have exponents
 template <typename T>
-static void head_copy(const void *src, const float *scale, int64_t R, const HeadArgs &h, bf16 *dst, int64_t part, hipStream_t s)
+static void head_copies(const Copy *of, int n, const HeadArgs &h, int number, uint32_t *largest, hipStream_t s)
 {
-    const int64_t pieces = R * (h.ld / 8);
-    if (pieces > 0)
-        hipLaunchKernelGGL((head_parts<T>), dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, s,
-                           static_cast<const T *>(src), scale, R, h.F, h.ld, dst, part);
+    Copies a{{of[0], of[n - 1]}, 0, h.F, h.ld};
+    int64_t blocks = 0;
+    for (int i = 0; i < n; i++) {
+        a.of[i].largest = largest + (number + i) * kMaxBlocks;
+        a.of[i].exponent = reinterpret_cast<int *>(largest + 3 * kMaxBlocks) + number + i;
+        if (i == 1) a.blocks0 = (int)blocks;
+        blocks += ceil_div(of[i].R * (h.ld / 8), 256);
+    }
+    if (n == 1) a.blocks0 = (int)blocks;
+    if (sizeof(T) == 4) hipLaunchKernelGGL(head_largest, dim3(n * kMaxBlocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((head_parts<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
 }
 
 // x and w as parts: copies into the workspace, or the arrays themselves
 template <typename T>
-static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs, bf16 *ws, hipStream_t s)
+static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs, bf16 *ws, uint32_t *largest, hipStream_t s)
 {
     h->ld = (int)parts_ld(h->F);
     h->part_x = h->V * h->ld;
     h->part_w = (int64_t)h->C * h->ld;
+    h->exponents = sizeof(T) == 4 ? reinterpret_cast<const int *>(largest + 3 * kMaxBlocks) : nullptr;
     if (parts_in_place<T>(h->F)) {
         h->x = static_cast<const bf16 *>(x);
         h->w = static_cast<const bf16 *>(w);
@@ -705,8 +813,10 @@ static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs
     }
     h->x = xs;
     h->w = ws;
-    head_copy<T>(x, nullptr, h->V, *h, xs, h->part_x, s);
-    head_copy<T>(w, nullptr, h->C, *h, ws, h->part_w, s);
+    const int64_t blocks = ceil_div(h->part_x / 8, 256) + ceil_div(h->part_w / 8, 256);
+    if (blocks > 0x7fffffffLL) return fail(JGAMD_ERR_SIZE, "linear_cross_entropy: V=%lld F=%d C=%d is too large", (long long)h->V, h->F, h->C);
+    const Copy of[2] = {{x, nullptr, h->V, xs, h->part_x, nullptr, nullptr}, {w, nullptr, h->C, ws, h->part_w, nullptr, nullptr}};
+    head_copies<T>(of, 2, *h, 0, largest, s);
     return launch_status("linear_cross_entropy");
 }
 
@@ -738,6 +848,7 @@ static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t re
     const HeadScratch<T> n(h.V, h.F, h.C, false);
     Carver carve(ws);
     bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w);
+    uint32_t *largest = carve.take<uint32_t>(n.largest);
     float2 *stats = carve.take<float2>(n.stats);
     float *at_label = carve.take<float>(n.at_label);
     double *block_sum = carve.take<double>(n.blocks);
@@ -745,7 +856,7 @@ static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t re
     const int mean = reduction == JGAMD_LOSS_MEAN ? 1 : 0;
     int blocks = 0;
     if (h.V > 0) {
-        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
+        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, largest, st)) return rc;
         const int ranges = head_ranges<T>(h.V, h.C);
         if (head_few<T>(h.V)) launch_stats<T, HeadFew<T>>(h, ranges, stats, at_label, st);
         else launch_stats<T, HeadShape<T>>(h, ranges, stats, at_label, st);
@@ -769,17 +880,19 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
     const HeadScratch<T> n(h.V, h.F, h.C, true);
     Carver carve(ws);
     bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w), *gx = carve.take<bf16>(n.gx);
+    uint32_t *largest = carve.take<uint32_t>(n.largest);
     float *scale = carve.take<float>(n.scale);
     bf16 *d = carve.take<bf16>(n.d);
     float *part = carve.take<float>(n.part), *part_b = carve.take<float>(n.part_b);
     float *acc_x = carve.take<float>(n.acc_x), *acc_w = carve.take<float>(n.acc_w), *acc_b = carve.take<float>(n.acc_b);
     if (h.V > 0)
-        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
+        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, largest, st)) return rc;
     if (h.V == 0) h.ld = (int)parts_ld(h.F);
     const bool per_row = reduction == JGAMD_LOSS_NONE;
     if (per_row && h.V > 0) {
         hipLaunchKernelGGL(head_row_scale, dim3((unsigned)ceil_div(h.V, 256)), dim3(256), 0, st, h, grad, scale);
-        if (dw) head_copy<T>(x, scale, h.V, h, gx, h.V * h.ld, st);
+        const Copy of{x, scale, h.V, gx, h.V * h.ld, nullptr, nullptr};
+        if (dw) head_copies<T>(&of, 1, h, 2, largest, st);
     }
     const int ldd = (int)s.classes + kPad;
     const int64_t part_d = s.rows * ldd;
@@ -802,6 +915,7 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
             if (dx && rows > 0) {
                 a.row_scale = per_row ? scale + row0 : nullptr;
                 a.p = h.w + (int64_t)c0 * h.ld, a.part_p = h.part_w;
+                a.exponent_p = h.exponents ? h.exponents + 1 : nullptr;
                 a.M = rows, a.K = classes;
                 a.splits = sum_splits<T>(s.rows, h.F, s.classes);
                 a.k_split = (int)(ceil_div(ceil_div(s.classes, a.splits), 64) * 64);
@@ -812,6 +926,7 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
             if (dw) {
                 a.p = (per_row ? gx : h.x) + row0 * h.ld, a.part_p = per_row ? h.V * h.ld : h.part_x;
                 a.row_scale = nullptr;
+                a.exponent_p = h.exponents ? h.exponents + (per_row ? 2 : 0) : nullptr;
                 a.M = classes, a.K = rows;
                 a.splits = sum_splits<T>(s.classes, h.F, s.rows);
                 a.k_split = (int)(ceil_div(ceil_div(s.rows, a.splits), 64) * 64);

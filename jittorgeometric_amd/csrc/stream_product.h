@@ -1,5 +1,5 @@
-// The products of tile_product.h for operands that lie in memory as bfloat16 parts on 16-byte
-// addresses: tiles go from memory to LDS directly (buffer_load ... lds), several steps ahead, and a
+// The products of tile_product.h for operands that lie in memory as 16-bit parts on 16-byte addresses
+// (one bfloat16, or two float16 whose three products a1b1 + a1b2 + a2b1 stand for one of floats): tiles go from memory to LDS directly (buffer_load ... lds), several steps ahead, and a
 // workgroup that owns several tiles keeps loading across their borders.
 //
 // A step is 32 or 64 values of k.  STAGES steps have room in LDS; while one is multiplied, the next
@@ -26,7 +26,7 @@ namespace jg {
 
 constexpr uint32_t kStreamRange = 0x40000000u;      // bytes a lane's offset may span; past it reads zero
 
-// One tile of the product: p[row][k] or p[k][row] as bfloat16 parts `part` elements apart.
+// One tile of the product: p[row][k] or p[k][row] as parts `part` elements apart.
 // kAlongK: ld and K multiples of 8; kAcrossK: ld and rows multiples of 8.  p, q on 16-byte addresses.
 struct StreamTile {
     const bf16 *p, *q;
@@ -38,6 +38,7 @@ struct StreamTile {
 
 template <int PARTS, int BN_, int BM_, int WN_, int WM_, int STEP_, int STAGES_> struct StreamShape {
     static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, kStep = STEP_, kStages = STAGES_, kParts = PARTS;
+    static_assert(PARTS == 1 || PARTS == 2, "one bfloat16 or two float16");
     static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
     static constexpr int FN = BN / WN / 16, FM = BM / WM / 16;
     static constexpr int kLoadsP = BN * kStep / 512 / kWaves, kLoadsQ = BM * kStep / 512 / kWaves;      // of a wavefront, step and part
@@ -158,6 +159,13 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
         }
     }
 
+    __device__ __forceinline__ static f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c)
+    {
+        typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+        if constexpr (S::kParts == 2)
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
     // the products of fragments i0 .. i1 - 1 of P, parts from the smallest products to the largest
     template <int PARTS>
     __device__ __forceinline__ static void multiply(f32x4 (&acc)[S::FN][S::FM], const bf16x8 (&fp)[S::kParts][S::FN],
@@ -171,7 +179,7 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
                 for (int i = i0; i < i1; i++)
 #pragma unroll
                     for (int j = 0; j < S::FM; j++)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[a][i], fq[sum - a][j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = mma(fp[a][i], fq[sum - a][j], acc[i][j]);
     }
 
     // Multiplies tiles 0 .. tiles - 1: tile(t) describes one (a StreamTile; cheap, called twice),
@@ -273,21 +281,18 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
                 };
                 auto step = [&](auto at_k) {
                     read(std::integral_constant<int, 0>(), at_k);
-                    if constexpr (S::kParts == 3) {
-                        read(std::integral_constant<int, 1>(), at_k);
-                        read(std::integral_constant<int, 2>(), at_k);
-                    }
+                    if constexpr (S::kParts == 2) read(std::integral_constant<int, 1>(), at_k);
                     if constexpr (S::kParts > 1 || PL == kAlongK) multiply<S::kParts>(acc, fp, fq, 0, S::FN);
                     if (SUMS != kNoSums) {
-                        const uint32_t one = 0x3f803f80u;      // two bfloat16 ones
+                        const uint32_t one = S::kParts == 2 ? 0x3c003c00u : 0x3f803f80u;      // two ones
                         const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one, one, one, one});
 #pragma unroll
                         for (int s = S::kParts - 1; s >= 0; s--)
 #pragma unroll
                             for (int i = 0; i < kSums; i++)
                                 sums[i] = SUMS == kSumP
-                                              ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[s][i], ones, sums[i], 0, 0, 0)
-                                              : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fq[s][i], sums[i], 0, 0, 0);
+                                              ? mma(fp[s][i], ones, sums[i])
+                                              : mma(ones, fq[s][i], sums[i]);
                     }
                 };
                 step(std::integral_constant<int, 0>());

@@ -94,21 +94,13 @@ template <> struct Eight<float> {
             if (i < n) (i < 4 ? a : b)[i & 3] = p[i];
     }
     __device__ __forceinline__ void clear() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
-    // the three parts, `part_bytes` apart in LDS, or `part` elements apart in memory
-    __device__ __forceinline__ void store(char *lds, int part_bytes) const
-    {
-        split([&](int s, u32x4 w) { *reinterpret_cast<u32x4 *>(lds + s * part_bytes) = w; });
-    }
-    __device__ __forceinline__ void store_parts(bf16 *out, int64_t part) const
-    {
-        split([&](int s, u32x4 w) { *reinterpret_cast<u32x4 *>(out + s * part) = w; });
-    }
     __device__ __forceinline__ void scale(float g)
     {
         if (g == 0.f) clear();
         else a *= g, b *= g;
     }
-    template <typename Put> __device__ __forceinline__ void split(Put &&put) const
+    // the three parts, `part_bytes` apart in LDS
+    __device__ __forceinline__ void store(char *lds, int part_bytes) const
     {
         float r[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 #pragma unroll
@@ -120,7 +112,7 @@ template <> struct Eight<float> {
                 r[2 * i] -= bf16_lo(w[i]);
                 r[2 * i + 1] -= bf16_hi(w[i]);
             }
-            put(s, w);
+            *reinterpret_cast<u32x4 *>(lds + s * part_bytes) = w;
         }
     }
 };

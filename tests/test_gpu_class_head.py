@@ -9,7 +9,13 @@ where d is rounded to bfloat16.  Gradients add that through |w|, |x| or 1, and (
 absolute terms for n summands; a result rounded to bfloat16 is off by 2^-8 of itself more.  Numbers
 under 2^-126 may be lost: float32 has no exponent for them.  An exponential and its product with g
 (|g| < 4 here, but for the scaled means, whose g is under 1) lose under 2^-124 together, a product with
-an entry of the other operand under 2^-126."""
+an entry of the other operand under 2^-126.
+
+float32 operands are held as two float16 parts of an array scaled so that its largest entry M lies in
+2^14 .. 2^15: two roundings to 11 bits leave 2^-24 of an entry (the 16 u above cover those of both factors
+and the product of the second parts), but float16's spacing ends at 2^-24, so that an entry is never held
+closer than half of that, 2^-25 2^-14 M < 2^-38 M.  A sum over k is off by 2^-38 (M_x sum |w| + M_w sum |x|)
+more, d (M = 1) by 2^-38 |g| more."""
 import math
 
 import pytest
@@ -21,6 +27,7 @@ pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
 TINY = 2.0 ** -124
+GRAIN = 2.0 ** -38
 DTYPES = [torch.float32, torch.bfloat16]
 
 
@@ -32,7 +39,10 @@ def reference(x, w, b, t, g, reduction):
     b = torch.zeros(C, dtype=torch.float64, device=x.device) if b is None else b.detach().double()
     z = torch.mm(x, w.t()) + b
     live = torch.isfinite(b)
+    grain = 0.0 if half else GRAIN
+    top = lambda v: float(v.abs().amax()) if v.numel() else 0.0  # noqa: E731
     D = (2 * F + 16) * U * (torch.mm(x.abs(), w.abs().t()) + torch.where(live, b.abs(), 0)).amax(1)
+    D = D + grain * (top(x) * w.abs().sum(1).amax() + top(w) * x.abs().sum(1))
     lse = torch.logsumexp(z, 1)
     ok = (t >= 0) & (t < C)
     lab = torch.where(ok, t, 0).long()
@@ -57,11 +67,13 @@ def reference(x, w, b, t, g, reduction):
     d.scatter_add_(1, lab[:, None], -torch.ones_like(at)[:, None])
     d = torch.where(ok[:, None], d * g[:, None], 0)
     dd = torch.where(ok[:, None], 3 * E[:, None] * p * g.abs()[:, None], 0) + (2.0 ** -8 if half else 4 * U) * d.abs() + TINY
+    dd = dd + torch.where(ok, grain * g.abs(), 0)[:, None]
     A = d.abs()
     ones = torch.ones(V, 1, dtype=torch.float64, device=x.device)
 
     def grad(left, leftd, leftabs, right, terms):
-        return torch.mm(left, right), torch.mm(leftd + (2 * terms + 16) * U * leftabs, right.abs()) + terms * TINY
+        tol = torch.mm(leftd + (2 * terms + 16) * U * leftabs, right.abs()) + terms * TINY
+        return torch.mm(left, right), tol + grain * top(right) * leftabs.sum(1, keepdim=True)
 
     # with one g a row dw takes g x, rounded to bfloat16 once more: 2^-8 of every term
     again = 2.0 ** -8 * A if half and reduction == "none" else 0
