@@ -137,13 +137,18 @@ def needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+# the current device's number without torch's checks around it, where this torch offers that
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 class on:
     """Makes `device` the current one for a launch (a stream belongs to its device); free where it
     already is."""
+    __slots__ = ("_guard",)
 
     def __init__(self, device):
         self._guard = None
-        if device.index is not None and device.index != torch.cuda.current_device():
+        if device.index is not None and device.index != _raw_device():
             self._guard = torch.cuda.device(device)
 
     def __enter__(self):

@@ -608,26 +608,22 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
         });
 }
 
-// grid: x = results / 1024 (of [M][N], then of [M])
+// grid: x = results / 256 (of [M][N], then of [M])
 template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a)
 {
-    const int64_t size = (int64_t)a.M * a.N, all = size + (a.out_b ? a.M : 0);
-    const float g = a.last && !a.row_scale ? sum_scale(a, 0, false) : 1.f, g_b = a.last && a.out_b ? sum_scale(a, 0, true) : 1.f;
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const int64_t e = (int64_t)blockIdx.x * 1024 + u * 256 + threadIdx.x;
-        if (e >= all) return;
-        const bool b = e >= size;
-        const int64_t at = b ? e - size : e, stride = b ? a.M : size;
-        const float *part = b ? a.part_b : a.part;
-        float *acc = b ? a.acc_b : a.acc;
-        float v = a.first ? 0.f : acc[at];
-        for (int k = 0; k < a.splits; k++) v += part[k * stride + at];
-        if (a.last) static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v * (b ? g_b : a.row_scale ? sum_scale(a, (int)(at / a.N), false) : g));
-        else acc[at] = v;
-    }
+    const int64_t size = (int64_t)a.M * a.N, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= size + (a.out_b ? a.M : 0)) return;
+    const bool b = e >= size;
+    const int64_t at = b ? e - size : e, stride = b ? a.M : size;
+    const float *part = (b ? a.part_b : a.part) + at;
+    float *acc = b ? a.acc_b : a.acc;
+    float v = a.first ? 0.f : acc[at];
+#pragma unroll 8
+    for (int k = 0; k < a.splits; k++) v += part[k * stride];
+    if (a.last)
+        static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v * sum_scale(a, a.row_scale ? (int)(at / a.N) : 0, b));
+    else acc[at] = v;
 }
-
 
 // g of every row: grad where the row has a label, else zero.  grid: x = rows / 256
 __global__ __launch_bounds__(256) void head_row_scale(HeadArgs a, const float *__restrict__ grad, float *__restrict__ scale)
@@ -675,10 +671,7 @@ __global__ __launch_bounds__(256) void head_bias(const bf16 *__restrict__ d, int
 
 // workgroups of a launch: as many as are resident at once
 template <typename S> constexpr int head_resident() { return kCus * (int)(160 * 1024 / S::kLds); }
-template <typename T> static unsigned head_grid(int64_t tiles)
-{
-    return (unsigned)std::min<int64_t>(tiles, head_resident<HeadShape<T>>());
-}
+template <typename S> static unsigned head_grid(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, head_resident<S>()); }
 
 // ranges of class tiles: as many as fill the chip once
 template <typename S> static int ranges_of(int64_t V, int C)
@@ -693,21 +686,33 @@ template <typename T> static int head_ranges(int64_t V, int C)
     return head_few<T>(V) ? ranges_of<HeadFew<T>>(V, C) : ranges_of<HeadShape<T>>(V, C);
 }
 
+// calls body(S()) with the shape of the tiles of a sum with N columns
+template <typename T, typename Body> static auto with_sum_shape(int64_t N, Body &&body)
+{
+    using Full = HeadShape<T>;
+    const int width = stream_width(N);
+    if (width == 64) return body(typename StreamOfWidth<Full::kParts, 64, Full::kStep>::S());
+    if (width == 128) return body(typename StreamOfWidth<Full::kParts, 128, Full::kStep>::S());
+    return body(Full());
+}
+
 // splits of a sum over K for an [M][N] result: the fewest (of at least 512 steps each, up to 32) that
 // leave under an eighth of the workgroups' turns empty, or the best there is
 template <typename T> static int sum_splits(int64_t M, int64_t N, int64_t K)
 {
-    using S = HeadShape<T>;
-    const int64_t tiles = ceil_div(M, S::BM) * ceil_div(N, S::BN), resident = head_resident<S>();
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(32, resident / tiles), K / 512));
-    int64_t best = 1;
-    double best_used = 0.0;
-    for (int64_t n = 1; n <= most; n++) {
-        const double used = (double)(tiles * n) / (double)(ceil_div(tiles * n, resident) * resident);
-        if (used > best_used + 0.02) best = n, best_used = used;
-        if (used >= 0.875) break;
-    }
-    return (int)best;
+    return with_sum_shape<T>(N, [&](auto shape) {
+        using S = decltype(shape);
+        const int64_t tiles = ceil_div(M, S::BM) * ceil_div(N, S::BN), resident = head_resident<S>();
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(32, resident / tiles), K / 512));
+        int64_t best = 1;
+        double best_used = 0.0;
+        for (int64_t n = 1; n <= most; n++) {
+            const double used = (double)(tiles * n) / (double)(ceil_div(tiles * n, resident) * resident);
+            if (used > best_used + 0.02) best = n, best_used = used;
+            if (used >= 0.875) break;
+        }
+        return (int)best;
+    });
 }
 
 struct Pieces {
@@ -822,13 +827,16 @@ static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs
 
 template <typename T, Layout QL, Sums SUMS> static int32_t launch_sum(const SumArgs &a, hipStream_t s)
 {
-    using S = HeadShape<T>;
-    raise_lds<&head_sum<T, S, QL, SUMS>>(S::kLds);
-    const unsigned grid = head_grid<T>(ceil_div(a.N, S::BN) * ceil_div(a.M, S::BM) * a.splits);
-    hipLaunchKernelGGL((head_sum<T, S, QL, SUMS>), dim3(grid), dim3(S::kThreads), S::kLds, s, a);
+    with_sum_shape<T>(a.N, [&](auto shape) {
+        using S = decltype(shape);
+        raise_lds<&head_sum<T, S, QL, SUMS>>(S::kLds);
+        const unsigned grid = head_grid<S>(ceil_div(a.N, S::BN) * ceil_div(a.M, S::BM) * a.splits);
+        hipLaunchKernelGGL((head_sum<T, S, QL, SUMS>), dim3(grid), dim3(S::kThreads), S::kLds, s, a);
+        return 0;
+    });
     if (a.splits > 1) {
         const int64_t all = (int64_t)a.M * a.N + (a.out_b ? a.M : 0);
-        hipLaunchKernelGGL((head_join<T>), dim3((unsigned)ceil_div(all, 1024)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((head_join<T>), dim3((unsigned)ceil_div(all, 256)), dim3(256), 0, s, a);
     }
     return launch_status("linear_cross_entropy_bwd");
 }
@@ -905,7 +913,7 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
             if (rows > 0) {
                 const PieceArgs a{h, lse, row0, rows, c0, classes, d, part_d, ldd};
                 raise_lds<&head_piece<T, S>>(S::kLds);
-                hipLaunchKernelGGL((head_piece<T, S>), dim3(head_grid<T>(ceil_div(classes, S::BN) * ceil_div(rows, S::BM))),
+                hipLaunchKernelGGL((head_piece<T, S>), dim3(head_grid<S>(ceil_div(classes, S::BN) * ceil_div(rows, S::BM))),
                                    dim3(S::kThreads), S::kLds, st, a);
                 if (int32_t rc = launch_status("linear_cross_entropy_bwd")) return rc;
             }

@@ -598,17 +598,24 @@ template <typename S> static unsigned stream_grid(int64_t tiles)
 // 256 x 128 results (two workgroups a compute unit, steps of 32) against 256 x 256 (one, steps of 64): 65521 rows,
 // 32 types, 1024 x 2048: 423 and 420 us against 380 and 358 (the two directions); 120011 rows, 256 x 256: 45, 38
 // against 42, 35
-using TypedStream = StreamShape<1, 256, 256, 2, 4, 64, 2>;
+template <int WIDTH> using TypedStream = typename StreamOfWidth<1, WIDTH, 64>::S;
+using GradOfFewK = StreamShape<1, 256, 64, 4, 1, 64, 2>;      // dW of up to 64 rows
 
-template <Layout WL> static int32_t launch_rows_stream(const GroupedArgs &a, hipStream_t s)
+template <typename S, Layout WL> static int32_t launch_rows_stream(const GroupedArgs &a, hipStream_t s)
 {
-    using S = TypedStream;
     const int64_t mtiles = (int64_t)a.M / S::BM + std::min<int64_t>(a.G, a.M) + 2;
     const int64_t tiles = mtiles * ceil_div(a.N, S::BN);
     if (tiles > 0x3fffffffLL) return fail(JGAMD_ERR_SIZE, "grouped_rows: M=%d N=%d G=%d is too large", a.M, a.N, a.G);
     raise_lds<&grouped_rows_stream<S, WL>>(S::kLds);
     hipLaunchKernelGGL((grouped_rows_stream<S, WL>), dim3(stream_grid<S>(tiles)), dim3(S::kThreads), S::kLds, s, a, (int)mtiles);
     return launch_status("grouped_rows");
+}
+template <Layout WL> static int32_t rows_stream(const GroupedArgs &a, hipStream_t s)
+{
+    const int width = stream_width(a.N);
+    if (width == 64) return launch_rows_stream<TypedStream<64>, WL>(a, s);
+    if (width == 128) return launch_rows_stream<TypedStream<128>, WL>(a, s);
+    return launch_rows_stream<TypedStream<256>, WL>(a, s);
 }
 
 template <typename T> static int32_t launch_thin(const GroupedArgs &a, bool transposed, hipStream_t s)
@@ -628,19 +635,26 @@ template <typename T> static int32_t rows_of_type(const GroupedArgs &a, bool tra
     if (a.M <= kThinMost && a.M <= (int64_t)kThinRows * a.G) return launch_thin<T>(a, transposed, s);
     if (sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 &&
         (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.out) & 15) == 0)
-        return transposed ? launch_rows_stream<kAlongK>(a, s) : launch_rows_stream<kAcrossK>(a, s);
+        return transposed ? rows_stream<kAlongK>(a, s) : rows_stream<kAcrossK>(a, s);
     using Wide = Shape<T, 128, 128, 2, 2>;
     using Narrow = Shape<T, 64, 128, 2, 2>;
     if (narrow_tiles(a.N)) return transposed ? launch_rows<T, Narrow, kAlongK>(a, s) : launch_rows<T, Narrow, kAcrossK>(a, s);
     return transposed ? launch_rows<T, Wide, kAlongK>(a, s) : launch_rows<T, Wide, kAcrossK>(a, s);
 }
 
-template <Sums SUMS> static void launch_grad_stream(const GradArgs &a, int64_t pieces, int64_t tiles, hipStream_t s)
+template <typename S> static int64_t launch_grad_stream(const GradArgs &a, int64_t pieces, hipStream_t s)
 {
-    using S = TypedStream;
-    raise_lds<&grouped_weight_grad_stream<S, SUMS>>(S::kLds);
-    hipLaunchKernelGGL((grouped_weight_grad_stream<S, SUMS>), dim3(stream_grid<S>(tiles)), dim3(S::kThreads), S::kLds, s, a,
-                       (int)pieces);
+    const int64_t tiles = ceil_div(a.N, S::BN) * ceil_div(a.K, S::BM) * pieces;
+    if (tiles > 0x3fffffffLL) return tiles;
+    const dim3 grid(stream_grid<S>(tiles)), threads(S::kThreads);
+    if (a.db) {
+        raise_lds<&grouped_weight_grad_stream<S, kSumP>>(S::kLds);
+        hipLaunchKernelGGL((grouped_weight_grad_stream<S, kSumP>), grid, threads, S::kLds, s, a, (int)pieces);
+    } else {
+        raise_lds<&grouped_weight_grad_stream<S, kNoSums>>(S::kLds);
+        hipLaunchKernelGGL((grouped_weight_grad_stream<S, kNoSums>), grid, threads, S::kLds, s, a, (int)pieces);
+    }
+    return tiles;
 }
 
 template <typename T, int BN, int BM> static int64_t launch_grad(const GradArgs &a, int64_t pieces, hipStream_t s)
@@ -658,11 +672,11 @@ template <typename T> static int32_t weight_grad_of_type(const GradArgs &a, hipS
     const bool stream = sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 && (((uintptr_t)a.x | (uintptr_t)a.dout) & 15) == 0;
     int64_t tiles;
     if (stream) {
-        tiles = ceil_div(a.N, TypedStream::BN) * ceil_div(a.K, TypedStream::BM) * pieces;
-        if (tiles <= 0x3fffffffLL) {
-            if (a.db) launch_grad_stream<kSumP>(a, pieces, tiles, s);
-            else launch_grad_stream<kNoSums>(a, pieces, tiles, s);
-        }
+        const int width = stream_width(a.N);
+        if (a.K <= 64 && width > 64) tiles = launch_grad_stream<GradOfFewK>(a, pieces, s);
+        else if (width == 64) tiles = launch_grad_stream<TypedStream<64>>(a, pieces, s);
+        else if (width == 128) tiles = launch_grad_stream<TypedStream<128>>(a, pieces, s);
+        else tiles = launch_grad_stream<TypedStream<256>>(a, pieces, s);
     } else if (narrow_tiles(a.N)) {
         tiles = narrow_tiles(a.K) ? launch_grad<T, 64, 64>(a, pieces, s) : launch_grad<T, 64, 128>(a, pieces, s);
     } else {

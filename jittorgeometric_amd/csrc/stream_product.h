@@ -73,6 +73,26 @@ template <int OFFSET, int LINE> __device__ __forceinline__ void fragments_across
         out[i] = __builtin_bit_cast(bf16x8, u32x4{v[2 * i][0], v[2 * i][1], v[2 * i + 1][0], v[2 * i + 1][1]});
 }
 
+// Widths of tiles for an n that is a fraction of 256: 64 (two workgroups a compute unit), 128, 256.  The
+// fewer n a tile has, the more of its time goes into loading Q: a column of a tile of 128 is taken to
+// cost 1.1, of 64 1.25 of one of 256.
+inline int stream_width(int64_t n)
+{
+    const double full = (double)((n + 255) / 256 * 256), half = 1.1 * (double)((n + 127) / 128 * 128),
+                 quarter = 1.25 * (double)((n + 63) / 64 * 64);
+    return quarter <= half && quarter <= full ? 64 : half <= full ? 128 : 256;
+}
+template <int PARTS, int WIDTH, int STEP> struct StreamOfWidth;
+template <int PARTS, int STEP> struct StreamOfWidth<PARTS, 256, STEP> {
+    using S = StreamShape<PARTS, 256, 256, 2, 4, STEP, 2>;
+};
+template <int PARTS, int STEP> struct StreamOfWidth<PARTS, 128, STEP> {
+    using S = StreamShape<PARTS, 128, 256, 2, 4, STEP, 3>;
+};
+template <int PARTS, int STEP> struct StreamOfWidth<PARTS, 64, STEP> {
+    using S = StreamShape<PARTS, 64, 256, 1, 4, STEP, 2>;
+};
+
 template <int N> __device__ __forceinline__ void wait_all_but()
 {
     // vmcnt <= N and lgkmcnt == 0 (expcnt is not waited for)
