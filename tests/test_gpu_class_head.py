@@ -295,7 +295,7 @@ def test_replays_as_a_graph_and_on_another_stream():
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
         for _ in range(2):
-            side = [v.clone() for v in step()]
+            side = [v.detach().clone() for v in step()]
     torch.cuda.current_stream().wait_stream(s)
     for a, c in zip(side, step()):
         assert torch.equal(a, c)
@@ -307,7 +307,7 @@ def test_replays_as_a_graph_and_on_another_stream():
             x.copy_(torch.randn_like(x))
             t.copy_(torch.randint_like(t, 0, 3000))
         torch.cuda.synchronize()
-        want = [v.clone() for v in step()]
+        want = [v.detach().clone() for v in step()]
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()

@@ -275,7 +275,7 @@ def test_forward_and_backward_replay_as_a_graph_and_on_another_stream():
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
         for _ in range(2):
-            side = [t.clone() for t in step()]
+            side = [t.detach().clone() for t in step()]
     torch.cuda.current_stream().wait_stream(s)
     for a, c in zip(side, step()):
         assert torch.equal(a, c)
@@ -287,7 +287,7 @@ def test_forward_and_backward_replay_as_a_graph_and_on_another_stream():
             x.copy_(torch.randn_like(x))
             dout.copy_(torch.randn_like(dout))
         torch.cuda.synchronize()
-        want = [t.clone() for t in step()]
+        want = [t.detach().clone() for t in step()]
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
