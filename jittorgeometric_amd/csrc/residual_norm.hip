@@ -303,6 +303,13 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
         Four<T> x[C], y[C], gate[C], dh[C], ds[C];
         float rs, ry;
     };
+    // whether no lane of this wavefront holds the row's ragged end
+    bool even[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int n = a.F - (c * L + lane) * V;
+        even[c] = __all(n >= V || n <= 0);
+    }
     auto read = [&](int64_t row) {
         Row r;
         const bool mine = row < a.R;
@@ -310,15 +317,20 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
 #pragma unroll
         for (int c = 0; c < C; c++) {
             const int f = (c * L + lane) * V, left = mine ? a.F - f : 0;
-            r.x[c] = load_four<WHOLE>(x + base + f, left);
             r.y[c].clear();
             r.gate[c].clear();
             r.dh[c].clear();
             r.ds[c].clear();
-            if (y) r.y[c] = load_four<WHOLE>(y + base + f, left);
-            if (gate) r.gate[c] = load_four<WHOLE>(gate + base + f, left);
-            if (dh) r.dh[c] = load_four<WHOLE>(dh + base + f, left);
-            if (ds) r.ds[c] = load_four<WHOLE>(ds + base + f, left);
+            auto load = [&](auto whole) {
+                constexpr bool W = decltype(whole)::value;
+                r.x[c] = load_four<W>(x + base + f, left);
+                if (y) r.y[c] = load_four<W>(y + base + f, left);
+                if (gate) r.gate[c] = load_four<W>(gate + base + f, left);
+                if (dh) r.dh[c] = load_four<W>(dh + base + f, left);
+                if (ds) r.ds[c] = load_four<W>(ds + base + f, left);
+            };
+            if (WHOLE || even[c]) load(std::true_type());
+            else load(std::false_type());
         }
         r.rs = mine ? a.rs[row] : 0.f;
         r.ry = mine && post ? a.ry[row] : 1.f;
@@ -327,9 +339,8 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
     // every wavefront takes the same number of turns: the reductions of wide rows have barriers.  What a
     // lane holds past the row's end, or past the last row, is zero and adds zero.  The next row is read
     // while this one is worked on (rows of 1024 bfloat16: 1192 -> 896 us for 262144 of them), but not
-    // where that costs more than it brings: rows with a ragged end (1001 floats: 78 us without, 97 with)
-    // and the widest, whose registers would spill.
-    constexpr bool kAhead = WHOLE && C < 4;
+    // in the widest, whose registers would spill more.
+    constexpr bool kAhead = C < 4;
     const int64_t stride = (int64_t)gridDim.x * groups;
     Row next = read((int64_t)blockIdx.x * groups + group);
     for (int64_t row0 = (int64_t)blockIdx.x * groups; row0 < a.R; row0 += stride) {
@@ -393,9 +404,14 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
                 sum_p[c][i] += dv * u;
                 sum_s[c][i] += xg * up;
             }
-            if (a.dx) store_vec<WHOLE>(static_cast<T *>(a.dx) + base + f, left[c], t[c]);
-            if (BLOCK && a.dy) store_vec<WHOLE>(static_cast<T *>(a.dy) + base + f, left[c], dy);
-            if (BLOCK && a.dgate) store_vec<WHOLE>(static_cast<T *>(a.dgate) + base + f, left[c], dg);
+            auto store = [&](auto whole) {
+                constexpr bool W = decltype(whole)::value;
+                if (a.dx) store_vec<W>(static_cast<T *>(a.dx) + base + f, left[c], t[c]);
+                if (BLOCK && a.dy) store_vec<W>(static_cast<T *>(a.dy) + base + f, left[c], dy);
+                if (BLOCK && a.dgate) store_vec<W>(static_cast<T *>(a.dgate) + base + f, left[c], dg);
+            };
+            if (WHOLE || even[c]) store(std::true_type());
+            else store(std::false_type());
         }
         if (!kAhead && row0 + stride < a.R) next = read(row + stride);
     }
