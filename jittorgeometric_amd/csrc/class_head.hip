@@ -59,7 +59,8 @@ template <typename T> using HeadFew = typename HeadFewOf<T>::S;
 // all of a's 24 bits but the last; e brings the array's largest entry to 2^14 .. 2^15.  Dropping a2 b2
 // (under 2^-24 of a b) leaves three products, half of what three bfloat16 parts take.  float16 ends at
 // 2^-24: an entry under 2^-17 of the array's largest keeps an absolute precision of 2^-39 of that largest
-// instead of 24 bits of its own.  d is stored times 2^15 (|d| <= 1): probabilities under 2^-17 keep 2^-40.
+// instead of 24 bits of its own: the logits of every row are off by 2^-39 of what the largest entry gives,
+// which is nothing to a softmax unless that row's own logits reach 10^5.  d is stored times 2^15 (|d| <= 1): probabilities under 2^-17 keep 2^-40.
 constexpr int kDExponent = 15;
 constexpr int kMaxBlocks = 256;      // workgroups that look for an array's largest entry
 
@@ -75,11 +76,13 @@ struct HeadArgs {
     int F, C;
 };
 
-__device__ __forceinline__ int64_t head_label(const HeadArgs &a, int64_t row)
+// the label of a row, -1 where it names no class
+__device__ __forceinline__ int64_t label_in(const int32_t *y32, const int64_t *y64, int C, int64_t row)
 {
-    const int64_t y = a.y64 ? a.y64[row] : (int64_t)a.y32[row];
-    return y >= 0 && y < a.C ? y : -1;
+    const int64_t y = y64 ? y64[row] : (int64_t)y32[row];
+    return y >= 0 && y < C ? y : -1;
 }
+__device__ __forceinline__ int64_t head_label(const HeadArgs &a, int64_t row) { return label_in(a.y32, a.y64, a.C, row); }
 
 // 2^-(e1 + e2), as near as a float comes
 __device__ __forceinline__ float unscale(int e1, int e2) { return ldexpf(1.f, min(max(-(e1 + e2), -126), 127)); }
@@ -158,10 +161,12 @@ template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int
 }
 
 // One array to be laid out as parts: [R][F] of T to [R][ld], zero behind F; rows times scale[R] unless
-// that is NULL (a row times zero is zero whatever it holds).
+// that is NULL (a row times zero is zero whatever it holds), or, with `labelled`, zero without a label:
+// what a padded row holds neither enters dW as 0 x NaN nor sets the array's exponent.
 struct Copy {
     const void *src;
     const float *scale;
+    int labelled;
     int64_t R;
     bf16 *dst;
     int64_t part;            // elements between the parts
@@ -170,21 +175,24 @@ struct Copy {
 };
 struct Copies {
     Copy of[2];
+    const int32_t *y32;
+    const int64_t *y64;
     int blocks0;             // workgroups of the first; the others have the second
-    int F, ld;
+    int F, ld, C;
 };
 
 // piece `id` of 8 entries of an array
-template <typename T> __device__ __forceinline__ Eight<T> copy_piece(const Copy &c, int F, int ld, int64_t id)
+template <typename T> __device__ __forceinline__ Eight<T> copy_piece(const Copies &a, const Copy &c, int64_t id)
 {
-    const int across = ld / 8;
+    const int across = a.ld / 8;
     const int64_t row = id / across;
     const int at = (int)(id - row * across) * 8;
     Eight<T> e;
-    const T *src = static_cast<const T *>(c.src) + row * F + at;
-    if (at + 8 <= F) e.load(src);
-    else e.load_some(src, F - at);
+    const T *src = static_cast<const T *>(c.src) + row * a.F + at;
+    if (at + 8 <= a.F) e.load(src);
+    else e.load_some(src, a.F - at);
     if (c.scale) e.scale(c.scale[row]);
+    if (c.labelled && label_in(a.y32, a.y64, a.C, row) < 0) e.clear();
     return e;
 }
 
@@ -202,7 +210,7 @@ __global__ __launch_bounds__(256) void head_largest(Copies a)
     };
 #pragma unroll 4
     for (int64_t id = (int64_t)block * 256 + threadIdx.x; id < pieces; id += kMaxBlocks * 256) {
-        const Eight<float> e = copy_piece<float>(c, a.F, a.ld, id);
+        const Eight<float> e = copy_piece<float>(a, c, id);
 #pragma unroll
         for (int i = 0; i < 4; i++) see(e.a[i]), see(e.b[i]);
     }
@@ -235,7 +243,7 @@ template <typename T> __global__ __launch_bounds__(256) void head_parts(Copies a
     }
     const int64_t id = (int64_t)block * 256 + threadIdx.x;
     if (id >= c.R * (a.ld / 8)) return;
-    const Eight<T> e = copy_piece<T>(c, a.F, a.ld, id);
+    const Eight<T> e = copy_piece<T>(a, c, id);
     if constexpr (sizeof(T) == 4) {
         float v[8];
 #pragma unroll
@@ -790,7 +798,7 @@ static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int3
 template <typename T>
 static void head_copies(const Copy *of, int n, const HeadArgs &h, int number, uint32_t *largest, hipStream_t s)
 {
-    Copies a{{of[0], of[n - 1]}, 0, h.F, h.ld};
+    Copies a{{of[0], of[n - 1]}, h.y32, h.y64, 0, h.F, h.ld, h.C};
     int64_t blocks = 0;
     for (int i = 0; i < n; i++) {
         a.of[i].largest = largest + (number + i) * kMaxBlocks;
@@ -820,7 +828,8 @@ static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs
     h->w = ws;
     const int64_t blocks = ceil_div(h->part_x / 8, 256) + ceil_div(h->part_w / 8, 256);
     if (blocks > 0x7fffffffLL) return fail(JGAMD_ERR_SIZE, "linear_cross_entropy: V=%lld F=%d C=%d is too large", (long long)h->V, h->F, h->C);
-    const Copy of[2] = {{x, nullptr, h->V, xs, h->part_x, nullptr, nullptr}, {w, nullptr, h->C, ws, h->part_w, nullptr, nullptr}};
+    const Copy of[2] = {{x, nullptr, 1, h->V, xs, h->part_x, nullptr, nullptr},
+                        {w, nullptr, 0, h->C, ws, h->part_w, nullptr, nullptr}};
     head_copies<T>(of, 2, *h, 0, largest, s);
     return launch_status("linear_cross_entropy");
 }
@@ -897,10 +906,12 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
         if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, largest, st)) return rc;
     if (h.V == 0) h.ld = (int)parts_ld(h.F);
     const bool per_row = reduction == JGAMD_LOSS_NONE;
-    if (per_row && h.V > 0) {
-        hipLaunchKernelGGL(head_row_scale, dim3((unsigned)ceil_div(h.V, 256)), dim3(256), 0, st, h, grad, scale);
-        const Copy of{x, scale, h.V, gx, h.V * h.ld, nullptr, nullptr};
-        if (dw) head_copies<T>(&of, 1, h, 2, largest, st);
+    if (per_row && h.V > 0) hipLaunchKernelGGL(head_row_scale, dim3((unsigned)ceil_div(h.V, 256)), dim3(256), 0, st, h, grad, scale);
+    // what dW sums: x, times one g a row if there is one, rows without a label zero (32768 x 1024 bf16: 30 us of 9 ms)
+    const bool own_copy = per_row || parts_in_place<T>(h.F);
+    if (dw && own_copy && h.V > 0) {
+        const Copy of{x, per_row ? scale : nullptr, !per_row, h.V, gx, h.V * h.ld, nullptr, nullptr};
+        head_copies<T>(&of, 1, h, 2, largest, st);
     }
     const int ldd = (int)s.classes + kPad;
     const int64_t part_d = s.rows * ldd;
@@ -932,9 +943,9 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
                 if (int32_t rc = launch_sum<T, kAlongK, kNoSums>(a, st)) return rc;
             }
             if (dw) {
-                a.p = (per_row ? gx : h.x) + row0 * h.ld, a.part_p = per_row ? h.V * h.ld : h.part_x;
+                a.p = (own_copy ? gx : h.x) + row0 * h.ld, a.part_p = own_copy ? h.V * h.ld : h.part_x;
                 a.row_scale = nullptr;
-                a.exponent_p = h.exponents ? h.exponents + (per_row ? 2 : 0) : nullptr;
+                a.exponent_p = h.exponents ? h.exponents + (own_copy ? 2 : 0) : nullptr;
                 a.M = classes, a.K = rows;
                 a.splits = sum_splits<T>(s.classes, h.F, s.rows);
                 a.k_split = (int)(ceil_div(ceil_div(s.rows, a.splits), 64) * 64);

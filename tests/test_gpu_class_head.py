@@ -172,6 +172,26 @@ def test_rows_without_a_label(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("F", [32, 29])
+@pytest.mark.parametrize("left", [math.nan, math.inf, 3e38])
+def test_what_a_row_without_a_label_holds(dtype, reduction, F, left):
+    V, C = 90, 150
+    x, w, b, t, g = inputs(V, F, C, dtype)
+    out = ~((t >= 0) & (t < C))
+    assert out.any()
+    g = g if reduction == "none" else 1.0
+    with torch.no_grad():
+        x[out] = 0
+    want = run(x, w, b, t, g, reduction)
+    with torch.no_grad():
+        x[out] = left
+    got = run(x, w, b, t, g, reduction)
+    for k in ("loss", "dx", "dw", "db"):
+        assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_classes_masked_by_the_bias(dtype):
     x, w, b, t, g = inputs(70, 24, 300, dtype)
     with torch.no_grad():
