@@ -132,6 +132,13 @@ def stream_ptr(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def check_int32(who, *tensors):
+    """The C entries count with 32 bits; ctypes would cut a larger size off without a word."""
+    for t in tensors:
+        if max(t.shape, default=0) > 2**31 - 1:
+            raise JgamdError("%s: a size over 2^31 - 1: %s" % (who, tuple(t.shape)))
+
+
 def needs_grad(*tensors):
     """Whether a call with these inputs is recorded for a backward pass."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

@@ -84,7 +84,7 @@ __device__ __forceinline__ int64_t label_in(const int32_t *y32, const int64_t *y
 }
 __device__ __forceinline__ int64_t head_label(const HeadArgs &a, int64_t row) { return label_in(a.y32, a.y64, a.C, row); }
 
-// 2^-(e1 + e2), as near as a float comes
+// 2^-(e1 + e2), as near as a float comes: logits that need more are under 2^-80, or infinite
 __device__ __forceinline__ float unscale(int e1, int e2) { return ldexpf(1.f, min(max(-(e1 + e2), -126), 127)); }
 
 // (m, s): s exponentials relative to m.  An m of -inf holds nothing (s = 0).
@@ -542,17 +542,23 @@ struct SumArgs {
     int whole;          // four neighbouring values lie on an address that one access can take
 };
 
-__device__ __forceinline__ float sum_scale(const SumArgs &a, int m, bool sum_of_q)
+// what a sum is multiplied by: 2^down, which alone may be no float, then g
+struct SumScale {
+    int down;
+    float g;
+    __device__ __forceinline__ float of(float v) const { return ldexpf(v, down) * g; }
+};
+__device__ __forceinline__ SumScale sum_scale(const SumArgs &a, int m, bool sum_of_q)
 {
-    const float down = a.exponent_p ? unscale(kDExponent, sum_of_q ? 0 : *a.exponent_p) : 1.f;
-    if (a.row_scale) return down * a.row_scale[m];
-    if (!a.grad) return down;
-    if (!a.count) return down * a.grad[0];
-    return a.count[0] > 0 ? down * (a.grad[0] / (float)a.count[0]) : 0.f;      // no row counts: every sum is zero
+    const int down = a.exponent_p ? -kDExponent - (sum_of_q ? 0 : *a.exponent_p) : 0;
+    if (a.row_scale) return {down, a.row_scale[m]};
+    if (!a.grad) return {down, 1.f};
+    if (!a.count) return {down, a.grad[0]};
+    return {down, a.count[0] > 0 ? a.grad[0] / (float)a.count[0] : 0.f};      // no row counts: every sum is zero
 }
 
 template <typename T>
-__device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc, int64_t at, f32x4 v, int n, float g)
+__device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc, int64_t at, f32x4 v, int n, const SumScale &scale)
 {
     if (!a.first) {
         if (a.whole && n >= 4) v += *reinterpret_cast<const f32x4 *>(acc + at);
@@ -562,7 +568,7 @@ __device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc,
                 if (r < n) v[r] += acc[at + r];
         }
     }
-    if (a.last) store4<T>(static_cast<T *>(out) + at, v * g, n, a.whole);
+    if (a.last) store4<T>(static_cast<T *>(out) + at, f32x4{scale.of(v[0]), scale.of(v[1]), scale.of(v[2]), scale.of(v[3])}, n, a.whole);
     else store4<float>(acc + at, v, n, a.whole);
 }
 
@@ -599,7 +605,7 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
             for (int j = 0; j < S::FM; j++) {
                 const int m = m0 + Product::m_of(j);
                 if (m >= a.M) continue;
-                const float g = a.splits > 1 ? 1.f : sum_scale(a, m, false);
+                const SumScale scale = a.splits > 1 ? SumScale{0, 1.f} : sum_scale(a, m, false);
                 if (SUMS == kSumQ && n0 == 0 && Product::n_of(0) == 0) {
                     if (a.splits > 1) a.part_b[(int64_t)split * a.M + m] = sums[j][0];
                     else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1, sum_scale(a, m, true));
@@ -610,7 +616,7 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
                     if (n >= a.N) continue;
                     const int64_t at = (int64_t)m * a.N + n;
                     if (a.splits > 1) store4<float>(a.part + (int64_t)split * a.M * a.N + at, acc[i][j], a.N - n, a.whole);
-                    else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n, g);
+                    else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n, scale);
                 }
             }
         });
@@ -629,7 +635,7 @@ template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a
 #pragma unroll 8
     for (int k = 0; k < a.splits; k++) v += part[k * stride];
     if (a.last)
-        static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v * sum_scale(a, a.row_scale ? (int)(at / a.N) : 0, b));
+        static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(sum_scale(a, a.row_scale ? (int)(at / a.N) : 0, b).of(v));
     else acc[at] = v;
 }
 
@@ -907,7 +913,7 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
     if (h.V == 0) h.ld = (int)parts_ld(h.F);
     const bool per_row = reduction == JGAMD_LOSS_NONE;
     if (per_row && h.V > 0) hipLaunchKernelGGL(head_row_scale, dim3((unsigned)ceil_div(h.V, 256)), dim3(256), 0, st, h, grad, scale);
-    // what dW sums: x, times one g a row if there is one, rows without a label zero (32768 x 1024 bf16: 30 us of 9 ms)
+    // what dW sums: x, times one g a row if there is one, rows without a label zero (7 us of 9 ms for bf16)
     const bool own_copy = per_row || parts_in_place<T>(h.F);
     if (dw && own_copy && h.V > 0) {
         const Copy of{x, per_row ? scale : nullptr, !per_row, h.V, gx, h.V * h.ld, nullptr, nullptr};

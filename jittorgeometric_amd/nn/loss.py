@@ -154,6 +154,7 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
         raise _lib.JgamdError("linear_cross_entropy: bias must be [%d], got %s" % (weight.shape[0], tuple(bias.shape)))
     if reduction not in _REDUCTIONS:
         raise _lib.JgamdError("linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
+    _lib.check_int32("linear_cross_entropy", x, weight)
     _lib.dtype_code(x.dtype)
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.dtype != x.dtype:

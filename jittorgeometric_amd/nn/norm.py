@@ -58,6 +58,7 @@ def _apply(who, x, y, weight, post_weight, gate, scale, eps):
     _lib.require_gpu(x, y, weight, post_weight, gate, scale)
     if x.dim() != 2 or x.shape[1] == 0:
         raise _lib.JgamdError("%s: x must be [rows, features], got %s" % (who, tuple(x.shape)))
+    _lib.check_int32(who, x)
     _lib.dtype_code(x.dtype)
     F = x.shape[1]
     for name, t, shape in (("y", y, tuple(x.shape)), ("gate", gate, tuple(x.shape)), ("weight", weight, (F,)),

@@ -75,6 +75,7 @@ def grouped_rows(x, weight, offsets, bias=None):
     if bias is not None and tuple(bias.shape) != (weight.shape[0], weight.shape[2]):
         raise _lib.JgamdError("grouped_rows: bias must be [types, Fout] = [%d, %d], got %s"
                               % (weight.shape[0], weight.shape[2], tuple(bias.shape)))
+    _lib.check_int32("grouped_rows", x, weight)
     _lib.dtype_code(x.dtype)
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.dtype != x.dtype:

@@ -214,6 +214,16 @@ def test_large_logits():
     assert torch.isfinite(got["loss"]).all()
 
 
+@pytest.mark.parametrize("by_x,by_w", [(0, -105), (-105, 0), (-70, -70), (100, -110), (-110, 100)])
+def test_operands_far_from_one(by_x, by_w):
+    x, w, b, t, g = inputs(60, 32, 200, torch.float32)
+    with torch.no_grad():
+        x *= 2.0 ** by_x
+        w *= 2.0 ** by_w
+    for reduction, up in (("none", g), ("mean", 1.0)):
+        compare(x, w, b, t, up, reduction)
+
+
 def test_a_bad_row_stays_alone():
     x, w, b, t, g = inputs(140, 36, 260, torch.float32, unlabelled=False)
     want = run(x, w, b, t, g, "none")

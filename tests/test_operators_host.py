@@ -139,3 +139,10 @@ def test_linear_cross_entropy_arguments(lib):
     # the scratch does not grow with rows * classes
     assert size(1 << 20, 256, 1 << 20, 1, 1, ctypes.byref(n)) == 0 and n.value < 3 << 30
     assert size(1 << 20, 256, 1 << 20, 1, 0, ctypes.byref(n)) == 0 and n.value < 1 << 30
+
+
+def test_sizes_past_32_bits_are_refused():
+    from jittorgeometric_amd import JgamdError, _lib
+    _lib.check_int32("f", torch.empty(2**31 - 1, 0), torch.empty(()))
+    with pytest.raises(JgamdError):
+        _lib.check_int32("f", torch.empty(3), torch.empty(0, 2**31))
