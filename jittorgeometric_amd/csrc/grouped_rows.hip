@@ -22,6 +22,7 @@ namespace jg {
 
 constexpr int kMaxTypes = 65535;      // the summing kernel's grid.y
 constexpr int kMaxWidth = 1 << 20;
+constexpr int kSumBlocks = 4096;      // of the summing kernel
 
 // exclusive prefix over the workgroup of `v`, combined by max (MAX) or by addition; the total in *total
 template <int THREADS, bool MAX> __device__ __forceinline__ int block_exclusive(int v, int *wave_totals, int *total)
@@ -486,7 +487,9 @@ template <typename S, Sums SUMS> __global__ __launch_bounds__(S::kThreads, 2) vo
 }
 
 // Adds the pieces of the types that have several, in order: workgroup y takes the y-th such type.
-// grid: x = results / 1024, y = as many such types as there can be
+// grid: x = blocks of 256 results (all, or kSumBlocks over y, each with every gridDim.x-th), y = as many such
+// types as there can be: most may not exist, as when every type fits a piece.  45 pieces of 256 x 256 results on
+// average, up to 100: 15 us with four results a thread and one strand
 template <typename T> __global__ __launch_bounds__(256) void grouped_weight_grad_sum(GradArgs a)
 {
     __shared__ int wave_totals[4];
@@ -529,22 +532,33 @@ template <typename T> __global__ __launch_bounds__(256) void grouped_weight_grad
     const int pieces = uniform(s_pieces);
     if (pieces == 0) return;
     const int64_t type = uniform(s_type), slot = uniform(s_slot), size = (int64_t)a.K * a.N;
-    // four neighbouring results a thread, eight pieces under way at a time
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    auto add = [&](const float *part, int64_t stride, int64_t at, int n, T *out) {
+    // Four neighbouring results a lane, eight pieces under way at a time; wavefront s takes pieces s, s + 4, ...
+    // and the four sums are added in order.
+    __shared__ f32x4 strands[3][kWave];
+    const int strand = wave_in_block(), lane = lane_id();
+    auto add = [&](const float *part, int64_t stride, int64_t block, T *out) {
+        const int64_t e = (block * kWave + lane) * 4;
+        const int n = (int)min((int64_t)4, stride - e);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (n >= 4 && stride % 4 == 0) {
-            const f32x4 *src = reinterpret_cast<const f32x4 *>(part + slot * stride + at);
+        if (n == 4 && stride % 4 == 0) {
+            const f32x4 *src = reinterpret_cast<const f32x4 *>(part + slot * stride + e);
 #pragma unroll 8
-            for (int p = 0; p < pieces; p++) v += src[p * (stride / 4)];
+            for (int p = strand; p < pieces; p += 4) v += src[p * (stride / 4)];
         } else {
             for (int r = 0; r < 4 && r < n; r++)
-                for (int p = 0; p < pieces; p++) v[r] += part[(slot + p) * stride + at + r];
+                for (int p = strand; p < pieces; p += 4) v[r] += part[(slot + p) * stride + e + r];
         }
-        store4<T>(out + at, v, n, a.whole && stride % 4 == 0);
+        __syncthreads();
+        if (strand > 0) strands[strand - 1][lane] = v;
+        __syncthreads();
+        if (strand > 0 || n <= 0) return;
+        for (int s = 0; s < 3; s++) v += strands[s][lane];
+        store4<T>(out + e, v, n, a.whole && stride % 4 == 0);
     };
-    if (e < size) add(a.part, size, e, (int)min((int64_t)4, size - e), static_cast<T *>(a.dw) + type * size);
-    if (a.db && e < a.N) add(a.part_b, a.N, e, (int)min((int64_t)4, a.N - e), static_cast<T *>(a.db) + type * a.N);
+    for (int64_t block = blockIdx.x; block * kWave * 4 < size; block += gridDim.x) {
+        add(a.part, size, block, static_cast<T *>(a.dw) + type * size);
+        if (a.db && block * kWave * 4 < a.N) add(a.part_b, a.N, block, static_cast<T *>(a.db) + type * a.N);
+    }
 }
 
 // Rows a piece of the weight gradient sums: so many that about three workgroups per compute unit
@@ -686,8 +700,10 @@ template <typename T> static int32_t weight_grad_of_type(const GradArgs &a, hipS
         return fail(JGAMD_ERR_SIZE, "grouped_rows_weight_grad: K=%d N=%d G=%d is too large", a.K, a.N, a.G);
     if (int32_t rc = launch_status("grouped_rows_weight_grad")) return rc;
     if (a.M <= a.piece) return 0;
-    const unsigned gx = (unsigned)ceil_div((int64_t)a.K * a.N, 1024);
-    hipLaunchKernelGGL((grouped_weight_grad_sum<T>), dim3(gx, (unsigned)std::min(a.G, a.M / a.piece)), dim3(256), 0, s, a);
+    const unsigned types = (unsigned)std::min(a.G, a.M / a.piece);
+    const int64_t blocks = ceil_div((int64_t)a.K * a.N, 4 * kWave);
+    const unsigned gx = (unsigned)std::min<int64_t>(blocks, std::max<int64_t>(64, kSumBlocks / types));
+    hipLaunchKernelGGL((grouped_weight_grad_sum<T>), dim3(gx, types), dim3(256), 0, s, a);
     return launch_status("grouped_rows_weight_grad");
 }
 
