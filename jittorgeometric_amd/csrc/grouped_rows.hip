@@ -249,7 +249,7 @@ template <typename S, Layout WL> __global__ __launch_bounds__(S::kThreads, 2) vo
 // Few rows: the weights are read once and multiplied on the vector unit.  A tile of 128 rows holds a
 // handful, its steps follow one another a memory latency each, and reading the weights is all there is
 // to do: here every wavefront asks for its share of them at once.  kThinRows rows of x stand in LDS as
-// floats.  48 rows of 16 types, 256 x 256 floats: 20.6 us with tiles, 6 like this.
+// floats.  48 rows of 16 types, 256 x 256 floats: 20.6 us with tiles, 7.9 like this.
 constexpr int kThinRows = 8;
 constexpr int kThinMost = 128;       // rows of a call, at most
 constexpr int kThinSteps = 512;      // of k in LDS at a time

@@ -136,10 +136,14 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
     [classes] or None, all float32 or all bfloat16; target [rows], int32 or int64.  Rows whose label
     lies outside [0, classes) are left out of the mean, have loss 0 and get a zero gradient.
     reduction: "mean" over the rows with a label (NaN when there is none), "sum" or "none" ([rows]);
-    the loss is float32.  A class may be masked with a bias of -inf.  Products are summed in float32;
-    a float32 product keeps float32's 24 bits, but an entry of x or weight of 3.39e38 or more, an
-    infinity or a NaN makes the logits it enters NaN.  The gradient of the logits is rounded to the
-    type of x on its way into the gradients of x, weight and bias."""
+    the loss is float32.  A class may be masked with a bias of -inf.  What a row without a label holds
+    does not matter.
+
+    Products are summed in float32.  float32 entries keep 24 bits down to 2^-17 of the largest of
+    their array and 2^-39 of that largest below; an infinity or a NaN makes the logits it enters NaN.
+    The gradient of the logits is rounded to bfloat16 on its way into the other gradients, or, in
+    float32, held to 24 bits and at least 2^-40.  The scratch memory of a backward pass is up to a
+    gigabyte of those, float32 sums of the size of weight, and one or two copies of x."""
     _lib.require_gpu(x, weight, target, bias)
     if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
         raise _lib.JgamdError("linear_cross_entropy: x must be [rows, features] and weight [classes, features], got %s "
