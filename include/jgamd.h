@@ -9,7 +9,8 @@
  *   - extern "C", plain pointers and sizes; no C++ or torch types.
  *   - All data pointers are DEVICE pointers to contiguous arrays; indices are
  *     int32, values fp32 (the only combination the reference's hot path uses:
- *     data/data.py:103-106 casts edge_index to int32).
+ *     data/data.py:103-106 casts edge_index to int32), or, in entry points with
+ *     a `dtype`, fp32 or bfloat16 as it says.
  *   - Work is enqueued on `stream` (a hipStream_t passed as void*; NULL is the
  *     default stream).  Nothing synchronises the device; nothing allocates or
  *     frees device memory: scratch comes in through `ws` / `ws_bytes`, sized by
@@ -400,7 +401,8 @@ int32_t jgamd_dense_rows(const float *x1, const float *w1, int32_t K1, const flo
  * NULL; db needs dw) from grad ([1], or [V] with JGAMD_LOSS_NONE) and the
  * forward's lse and count.  The workspace (the query with backward = 1) holds
  * the gradient of the logits for a block of rows and a piece of the classes
- * (at most 1 GB), and fp32 sums.  Fixed order, no atomics.  bfloat16 x and w
+ * (at most 1 GB), fp32 sums and copies of x, w.  What rows without a label hold
+ * does not matter.  Fixed order, no atomics.  bfloat16 x and w
  * with F a multiple of 8 must lie on 16-byte addresses; fp32, and other widths,
  * are laid out anew in the workspace.
  * With few classes: jgamd_cross_entropy_fwd / _bwd on logits

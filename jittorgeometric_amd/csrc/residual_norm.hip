@@ -34,7 +34,9 @@ constexpr int kNormBlocks = 1024, kNormBlocksAlone = 2048;
 constexpr int kNormMaxWidth = 8192;
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);      // elements of a 16-byte access
-constexpr int kGradVec = 4;      // of the backward pass: eight arrays of a row in registers leave no room for more
+// of the backward pass: eight arrays of a row in registers leave no room for more (262144 rows of 1024 bfloat16:
+// 887 us, 1012 with 8)
+constexpr int kGradVec = 4;
 
 // V consecutive elements as floats; `n` of them exist (the rest read as zero, are not written).
 // WHOLE: rows are whole vectors, n is at least V or nothing exists.
