@@ -190,7 +190,7 @@ __device__ __forceinline__ int first_tile()
 
 template <typename S, Layout WL> __global__ __launch_bounds__(S::kThreads, 2) void grouped_rows_stream(GroupedArgs a, int mtiles)
 {
-    using Product = StreamProduct<S, WL, kAlongK>;
+    using Product = StreamProduct<S, WL, kAlongK, true>;      // results in pairs: 16-byte stores
     extern __shared__ __align__(16) char lds[];
     __shared__ Run runs[kRunsKept];
     const int ntiles = (a.N + S::BN - 1) / S::BN;
@@ -214,33 +214,30 @@ template <typename S, Layout WL> __global__ __launch_bounds__(S::kThreads, 2) vo
         [&](int t, f32x4(&acc)[S::FN][S::FM], f32x4 *) {
             const int type = uniform(runs[t].type), row0 = uniform(runs[t].row), rows = uniform(runs[t].rows);
             const int n0 = (number(t) % ntiles) * S::BN;
-            constexpr int kRun = Product::kPairs ? 2 : 1;      // fragments whose results are neighbours
+            bf16 *out = static_cast<bf16 *>(a.out) + (int64_t)row0 * a.N;
+            Eight<bf16> b[S::FN / 2];      // asked for before the first store: loads and stores end in order
 #pragma unroll
-            for (int i = 0; i < S::FN; i += kRun) {
-                const int n = n0 + Product::n_of(i);
-                if (n >= a.N) continue;
-                f32x4 b[kRun];
+            for (int i = 0; i < S::FN / 2; i++) b[i].clear();
+            if (a.bias && typed(type)) {
 #pragma unroll
-                for (int u = 0; u < kRun; u++) {
-                    b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (a.bias && typed(type)) {
-                        const bf16 *src = static_cast<const bf16 *>(a.bias) + (int64_t)type * a.N + n + 4 * u;
-#pragma unroll
-                        for (int r = 0; r < 4; r++) b[u][r] = to_float(src[r]);
-                    }
+                for (int i = 0; i < S::FN / 2; i++) {
+                    const int n = n0 + Product::n_of(2 * i);
+                    b[i].load(static_cast<const bf16 *>(a.bias) + (int64_t)type * a.N + (n < a.N ? n : 0));
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < S::FN; i += 2) {
+                const int n = n0 + Product::n_of(i);
+                const u32x4 e = b[i / 2].v;
+                const f32x4 b0 = {bf16_lo(e[0]), bf16_hi(e[0]), bf16_lo(e[1]), bf16_hi(e[1])};
+                const f32x4 b1 = {bf16_lo(e[2]), bf16_hi(e[2]), bf16_lo(e[3]), bf16_hi(e[3])};
 #pragma unroll
                 for (int j = 0; j < S::FM; j++) {
                     const int m = Product::m_of(j);
-                    if (m >= rows) continue;
-                    bf16 *out = static_cast<bf16 *>(a.out) + (int64_t)(row0 + m) * a.N + n;
-                    const f32x4 v = acc[i][j] + b[0];
-                    if constexpr (kRun == 2) {
-                        const f32x4 v2 = acc[i + 1][j] + b[1];
-                        *reinterpret_cast<u32x4 *>(out) = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
-                                                                pack_bf16(v2[0], v2[1]), pack_bf16(v2[2], v2[3])};
-                    } else
-                        *reinterpret_cast<u32x2 *>(out) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+                    const f32x4 v = acc[i][j] + b0, v2 = acc[i + 1][j] + b1;
+                    Product::store(out, ((uint32_t)m * (uint32_t)a.N + (uint32_t)n) * 2, m < rows && n < a.N,
+                                   u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v2[0], v2[1]),
+                                         pack_bf16(v2[2], v2[3])});
                 }
             }
         });

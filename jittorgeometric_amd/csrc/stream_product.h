@@ -13,10 +13,11 @@
 // The LDS image is in lines of 32 or 64 k, or of the tile's rows: a wavefront's load writes 1 KB in lane order, so the
 // permutation is applied to the address each lane asks for.
 //
-// Which row of P stands at which row of a 16 x 16 fragment is free.  With P along k the fragments
-// 2 i and 2 i + 1 of a wavefront share 32 rows such that a lane's two times four results are eight
+// Which row of P stands at which row of a 16 x 16 fragment is free.  In pairs the fragments 2 i and
+// 2 i + 1 of a wavefront share 32 rows such that a lane's two times four results are eight
 // neighbouring n: the four lanes of an m then store 64 contiguous bytes of bfloat16 at a time
-// instead of 32.  Across k the transposing reads take rows as they come, and n is natural.
+// instead of 32 (65521 rows of 32 types, 1024 x 2048: 402 -> 362 us).  Otherwise n is natural, four of a
+// lane and sixteen of a fragment: 64 contiguous bytes of floats.
 #pragma once
 #include <type_traits>
 
@@ -106,10 +107,10 @@ __device__ __forceinline__ void lds_barrier()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <typename S, Layout PL, Layout QL> struct StreamProduct {
+template <typename S, Layout PL, Layout QL, bool PAIRS = PL == kAlongK> struct StreamProduct {
     typedef __attribute__((address_space(3))) void lds_void;
     typedef __attribute__((address_space(3))) char lds_char;
-    static constexpr bool kPairs = PL == kAlongK;
+    static constexpr bool kPairs = PAIRS;
     static_assert(!kPairs || S::FN % 2 == 0, "fragments of P come in pairs");
 
     // n of register 0 of fragment i (the other three follow), m of fragment j
@@ -127,25 +128,25 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
 
     // The turn of a row's pieces: the eight rows that are read at a time (0 .. 7 of Q; 0 .. 3 and 8 .. 11
     // of P in pairs) fall on different banks.  Rows of 64 bytes alternate between two halves by themselves.
-    template <bool PAIRS> __device__ __forceinline__ static int turn(int row)
+    template <bool ROWS_IN_PAIRS> __device__ __forceinline__ static int turn(int row)
     {
-        const int eight = PAIRS ? (row & 3) | ((row >> 1) & 4) : row & 7;
+        const int eight = ROWS_IN_PAIRS ? (row & 3) | ((row >> 1) & 4) : row & 7;
         return kRowPieces == 8 ? eight : eight >> 1;
     }
     // fragment of 16 rows along k at step kk of a stage, this lane's row given
-    template <bool PAIRS> __device__ __forceinline__ static bf16x8 fragment_along(const char *lds, int row, int kk)
+    template <bool ROWS_IN_PAIRS> __device__ __forceinline__ static bf16x8 fragment_along(const char *lds, int row, int kk)
     {
         const int g = lane_id() >> 4;
-        return *reinterpret_cast<const bf16x8 *>(lds + row * (2 * S::kStep) + (((kk / 8 + g) ^ turn<PAIRS>(row)) << 4));
+        return *reinterpret_cast<const bf16x8 *>(lds + row * (2 * S::kStep) + (((kk / 8 + g) ^ turn<ROWS_IN_PAIRS>(row)) << 4));
     }
 
     // the addresses that this lane asks for, relative to the tile's (k = k0) corner
-    template <int BR, int LOADS, Layout LAY, bool PAIRS> struct Lane {
+    template <int BR, int LOADS, Layout LAY, bool ROWS_IN_PAIRS> struct Lane {
         uint32_t off[LOADS];
         __device__ __forceinline__ static int k_of(int u)
         {
             const int id = (wave_in_block() * LOADS + u) * kWave + lane_id();
-            if (LAY == kAlongK) return ((id % kRowPieces) ^ turn<PAIRS>(id / kRowPieces)) * 8;
+            if (LAY == kAlongK) return ((id % kRowPieces) ^ turn<ROWS_IN_PAIRS>(id / kRowPieces)) * 8;
             return id / (BR / 8);
         }
         __device__ __forceinline__ void place(int ld, int rows)
@@ -177,6 +178,13 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 r, (lds_void *)(lds + (wave_in_block() * LOADS + u) * 1024), 16, (int)off, 0, 0, 0);
         }
+    }
+
+    // 16 bytes to base + at where they exist
+    __device__ __forceinline__ static void store(bf16 *base, uint32_t at, bool exists, u32x4 v)
+    {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)kStreamRange, 0x00020000);
+        __builtin_amdgcn_raw_buffer_store_b128(v, r, (int)(exists ? at : kStreamRange), 0, 0);
     }
 
     __device__ __forceinline__ static f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c)
@@ -246,7 +254,9 @@ template <typename S, Layout PL, Layout QL> struct StreamProduct {
         const int line_row = 4 * (lane_id() & 3), line_k = 8 * (lane_id() >> 4) + ((lane_id() >> 2) & 3);
         const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char *)lds;
 #pragma unroll
-        for (int i = 0; i < S::FN; i++) across_p[i] = lds_at + Place<S::BN, S::kStep, kAcrossK>::at(wn + 16 * i + line_row, line_k);
+        for (int i = 0; i < S::FN; i++)
+            across_p[i] = lds_at + Place<S::BN, S::kStep, kAcrossK>::at(
+                                       kPairs ? wn + (i >> 1) * 32 + 2 * line_row + (i & 1) * 4 : wn + 16 * i + line_row, line_k);
 #pragma unroll
         for (int j = 0; j < S::FM; j++) across_q[j] = lds_at + S::kParts * S::kPartP + Place<S::BM, S::kStep, kAcrossK>::at(wm + 16 * j + line_row, line_k);
         int stage_at = 0;
