@@ -663,6 +663,9 @@ template <typename T> static int32_t rows_of_type(const GroupedArgs &a, bool tra
         return transposed ? rows_stream<kAlongK>(a, s) : rows_stream<kAcrossK>(a, s);
     using Wide = Shape<T, 128, 128, 2, 2>;
     using Narrow = Shape<T, 64, 128, 2, 2>;
+    using Small = Shape<T, 64, 64, 2, 2>;
+    if (((int64_t)a.M / 128 + std::min(a.G, a.M)) * ceil_div(a.N, 128) < 256)
+        return transposed ? launch_rows<T, Small, kAlongK>(a, s) : launch_rows<T, Small, kAcrossK>(a, s);
     if (narrow_tiles(a.N)) return transposed ? launch_rows<T, Narrow, kAlongK>(a, s) : launch_rows<T, Narrow, kAcrossK>(a, s);
     return transposed ? launch_rows<T, Wide, kAlongK>(a, s) : launch_rows<T, Wide, kAcrossK>(a, s);
 }
