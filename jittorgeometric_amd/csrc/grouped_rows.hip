@@ -658,13 +658,18 @@ template <typename T> static int32_t rows_of_type(const GroupedArgs &a, bool tra
 {
     // on average at most kThinRows rows a type; all of them of one type read its weight up to 16 times
     if (a.M <= kThinMost && a.M <= (int64_t)kThinRows * a.G) return launch_thin<T>(a, transposed, s);
-    if (sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 &&
-        (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.out) & 15) == 0)
+    // streaming tiles, unless too few of 256 x 256 to fill half of the chip: 3000 rows, 2000 -> 504 bfloat16,
+    // 24 of them: 57 us, 25 in tiles of 64 x 64 from registers; 6000 rows, 1024 -> 1024, 108 of them: 35 and 34
+    auto tiles_of = [&](int of) { return ((int64_t)a.M / of + std::min(a.G, a.M)) * ceil_div(a.N, of); };
+    if (sizeof(T) == 2 && a.K % 8 == 0 && a.N % 8 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.out) & 15) == 0 &&
+        tiles_of(256) >= 128)
         return transposed ? rows_stream<kAlongK>(a, s) : rows_stream<kAcrossK>(a, s);
     using Wide = Shape<T, 128, 128, 2, 2>;
     using Narrow = Shape<T, 64, 128, 2, 2>;
     using Small = Shape<T, 64, 64, 2, 2>;
-    if (((int64_t)a.M / 128 + std::min(a.G, a.M)) * ceil_div(a.N, 128) < 256)
+    // 150 rows, 2047 -> 100 floats, 2 tiles of 128 x 128: 144 us, 68 in those of 64 x 64; 20000 rows, 256 -> 256,
+    // 320 tiles: 29 and 26; 6000 rows, 1024 -> 1024, 400 tiles: 82 and 95
+    if (tiles_of(128) < 384)
         return transposed ? launch_rows<T, Small, kAlongK>(a, s) : launch_rows<T, Small, kAcrossK>(a, s);
     if (narrow_tiles(a.N)) return transposed ? launch_rows<T, Narrow, kAlongK>(a, s) : launch_rows<T, Narrow, kAcrossK>(a, s);
     return transposed ? launch_rows<T, Wide, kAlongK>(a, s) : launch_rows<T, Wide, kAcrossK>(a, s);

@@ -114,6 +114,19 @@ def test_weight_gradient_of_many_rows_is_summed_in_pieces(sizes, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("K,N", [(24, 40), (33, 47), (72, 264), (40, 128), (129, 100), (264, 72), (100, 129)])
+def test_more_rows_than_small_tiles_take(K, N, bias, dtype):
+    sizes = [20001, 0, 30011, 1, 127, 255]
+    x, w, b, dout = inputs(sum(sizes) + 7, K, N, len(sizes), dtype, bias=bias)
+    off = offsets_of(sizes, start=3)
+    got, want = run(x, w, b, off, dout), reference(x, w, b, off, dout)
+    names = ["out", "dx", "dw", "db"] if bias else ["out", "dx", "dw"]
+    for k in names:
+        check(got[k], want[k], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_no_type_are_zero_and_not_read(dtype):
     M, K, N = 300, 40, 24
     off = [7, 7, 150, 280]
