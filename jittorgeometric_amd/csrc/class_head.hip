@@ -359,6 +359,113 @@ __global__ __launch_bounds__(S::kThreads, 2) void head_stats(HeadArgs a, int ran
     }
 }
 
+// The statistics of a few rows of floats: w is read once, as it is, and multiplied on the vector unit, instead of
+// being laid out as parts for it.  kThinRows rows of x stand in LDS; sixteen lanes share four classes, 4 k a lane
+// and step.  The 32 sums of a group meet in a transposing reduction (16 + 8 + 4 + 2 shuffles) that leaves each
+// lane one class of two rows, whose running maximum and sum it keeps.  Bound by reading w for up to kThinRows
+// rows, by the vector unit beyond.  Whole calls, with parts and like this: 4 rows, 387 features, 48749 classes 79
+// and 25 us; 256 features, 50021 classes: 7 rows 46 and 22, 24 rows 47 and 43, 32 rows 47 and 43; 2000 features,
+// 20000 classes, 32 rows: 175 and 156.  (bfloat16 of odd widths, copied once: 8 rows 23 and 27, 32 rows 23 and 46.)
+// grid: x = blocks of kThinRows rows x ranges of tiles of 64 classes
+constexpr int kThinRows = 8;
+constexpr int kThinMost = 32;            // rows of a call, at most
+constexpr int kThinFeatures = 2048;      // 64 KB of x
+constexpr int kThinClasses = 64;
+
+// the first n (at most four, at least none) of p, zero behind them
+__device__ __forceinline__ f32x4 four(const float *p, int n)
+{
+    if (n >= 4) return *reinterpret_cast<const f32x4_at4 *>(p);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+        if (i < n) v[i] = p[i];
+    return v;
+}
+
+__global__ __launch_bounds__(256, 3) void head_thin(HeadArgs a, const float *__restrict__ x, const float *__restrict__ w,
+                                                    int ranges, int tiles_per_range, float2 *__restrict__ stats,
+                                                    float *__restrict__ at_label)
+{
+    extern __shared__ __align__(16) float xs[];      // [kThinRows][across]
+    __shared__ float2 joined[4][kThinRows];
+    const int across = (a.F + 63) / 64 * 64;
+    const int64_t row0 = (int64_t)(blockIdx.x / ranges) * kThinRows;
+    const int range = blockIdx.x % ranges, rows = (int)min((int64_t)kThinRows, a.V - row0);
+    for (int i = threadIdx.x; i < kThinRows * across; i += 256) {
+        const int r = i / across, k = i - r * across;
+        xs[i] = r < rows && k < a.F ? x[(row0 + r) * a.F + k] : 0.f;
+    }
+    __syncthreads();
+    const int lane = lane_id() & 15, group = wave_in_block() * 4 + (lane_id() >> 4);
+    const int r0 = ((lane >> 1) & 1) * 4 + (lane & 1) * 2;      // this lane's rows, r0 and r0 + 1
+    int label[2];
+    float m[2] = {-INFINITY, -INFINITY}, s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; u++) label[u] = r0 + u < rows ? (int)head_label(a, row0 + r0 + u) : -1;
+    const int tiles = (a.C + kThinClasses - 1) / kThinClasses;
+    const int last = min(tiles, (range + 1) * tiles_per_range);
+    for (int t = range * tiles_per_range; t < last; t++) {
+        const int c0 = t * kThinClasses + group * 4;
+        const float *from[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) from[c] = w + (int64_t)min(c0 + c, a.C - 1) * a.F;
+        float acc[4 * kThinRows] = {};
+#pragma unroll 2
+        for (int k = lane * 4; k < across; k += 64) {
+            f32x4 wv[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) wv[c] = four(from[c] + k, a.F - k);
+#pragma unroll
+            for (int r = 0; r < kThinRows; r++) {
+                const f32x4 xv = *reinterpret_cast<const f32x4 *>(xs + r * across + k);
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[c * kThinRows + r] = fmaf(wv[c][i], xv[i], acc[c * kThinRows + r]);
+            }
+        }
+        // class bits 1 and 0, row bits 2 and 1 go to lane bits 3, 2, 1, 0
+        auto fold = [&](auto lane_bit) {
+            constexpr int bit = decltype(lane_bit)::value, half = bit * kThinRows / 4;
+            const bool high = (lane & bit) != 0;
+#pragma unroll
+            for (int i = 0; i < half; i++) {
+                const float give = high ? acc[i] : acc[i + half], keep = high ? acc[i + half] : acc[i];
+                acc[i] = keep + __shfl_xor(give, bit, kWave);
+            }
+        };
+        fold(std::integral_constant<int, 8>());
+        fold(std::integral_constant<int, 4>());
+        fold(std::integral_constant<int, 2>());
+        fold(std::integral_constant<int, 1>());
+        const int cls = c0 + (lane >> 2);
+        const float b = a.bias && cls < a.C ? static_cast<const float *>(a.bias)[cls] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const float z = cls < a.C ? acc[u] + b : -INFINITY;
+            if (label[u] == cls) at_label[row0 + r0 + u] = z;
+            join_stats(m[u], s[u], z, cls < a.C ? 1.f : 0.f);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int o = 4; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(m[u], o, kWave), s2 = __shfl_xor(s[u], o, kWave);
+            join_stats(m[u], s[u], m2, s2);
+        }
+        if (lane_id() < 4) joined[wave_in_block()][r0 + u] = float2{m[u], s[u]};
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+        float2 v = joined[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < 4; k++) join_stats(v.x, v.y, joined[k][threadIdx.x].x, joined[k][threadIdx.x].y);
+        stats[(int64_t)range * a.V + row0 + threadIdx.x] = v;
+    }
+}
+
 // Joins a row's ranges to lse and loss, `lanes` lanes a row (a power of two up to 64), and adds the
 // workgroup's losses and labels in a fixed order; with one workgroup that is the result.
 // grid: x = rows / (kJoinThreads / lanes)
@@ -696,9 +803,17 @@ template <typename S> static int ranges_of(int64_t V, int C)
     const int64_t ranges = std::min<int64_t>(tiles, std::max<int64_t>(1, head_resident<S>() / blocks));
     return (int)ceil_div(tiles, ceil_div(tiles, ranges));
 }
-template <typename T> static bool head_few(int64_t V) { return V <= HeadFew<T>::BM; }
-template <typename T> static int head_ranges(int64_t V, int C)
+template <typename T> static bool head_thin_takes(int64_t V, int F)
 {
+    return sizeof(T) == 4 && V <= kThinMost && F <= kThinFeatures;
+}
+template <typename T> static bool head_few(int64_t V) { return V <= HeadFew<T>::BM; }
+template <typename T> static int head_ranges(int64_t V, int F, int C)
+{
+    if (head_thin_takes<T>(V, F)) {      // about four workgroups a compute unit
+        const int64_t tiles = ceil_div(C, kThinClasses), blocks = std::max<int64_t>(1, ceil_div(V, kThinRows));
+        return (int)ceil_div(tiles, ceil_div(tiles, std::min<int64_t>(tiles, 1024 / blocks)));
+    }
     return head_few<T>(V) ? ranges_of<HeadFew<T>>(V, C) : ranges_of<HeadShape<T>>(V, C);
 }
 
@@ -763,11 +878,13 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
     size_t part = 0, part_b = 0, acc_x = 0, acc_w = 0, acc_b = 0;     // float
     HeadScratch(int64_t V, int F, int C, bool backward)
     {
-        x = parts_elements<T>(V, F);
-        w = parts_elements<T>(C, F);
-        largest = sizeof(T) == 4 ? 3 * kMaxBlocks + 3 : 0;
+        if (backward || !head_thin_takes<T>(V, F)) {
+            x = parts_elements<T>(V, F);
+            w = parts_elements<T>(C, F);
+            largest = sizeof(T) == 4 ? 3 * kMaxBlocks + 3 : 0;
+        }
         if (!backward) {
-            stats = (size_t)head_ranges<T>(V, C) * V;
+            stats = (size_t)head_ranges<T>(V, F, C) * V;
             at_label = (size_t)V;
             blocks = (size_t)ceil_div(V, kJoinThreads / kWave);
             return;
@@ -881,9 +998,17 @@ static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t re
     const int mean = reduction == JGAMD_LOSS_MEAN ? 1 : 0;
     int blocks = 0;
     if (h.V > 0) {
-        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, largest, st)) return rc;
-        const int ranges = head_ranges<T>(h.V, h.C);
-        if (head_few<T>(h.V)) launch_stats<T, HeadFew<T>>(h, ranges, stats, at_label, st);
+        const int ranges = head_ranges<T>(h.V, h.F, h.C);
+        const bool thin = head_thin_takes<T>(h.V, h.F);
+        if (!thin)
+            if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, largest, st)) return rc;
+        if (thin) {
+            const size_t lds = sizeof(float) * kThinRows * (size_t)(ceil_div(h.F, 64) * 64);
+            raise_lds<&head_thin>(sizeof(float) * kThinRows * kThinFeatures);
+            hipLaunchKernelGGL(head_thin, dim3((unsigned)(ceil_div(h.V, kThinRows) * ranges)), dim3(256), lds, st, h,
+                               static_cast<const float *>(x), static_cast<const float *>(w), ranges,
+                               (int)ceil_div(ceil_div(h.C, kThinClasses), ranges), stats, at_label);
+        } else if (head_few<T>(h.V)) launch_stats<T, HeadFew<T>>(h, ranges, stats, at_label, st);
         else launch_stats<T, HeadShape<T>>(h, ranges, stats, at_label, st);
         int lanes = 1;      // four ranges a lane
         while (lanes < kWave && lanes * 4 < ranges) lanes *= 2;

@@ -172,6 +172,15 @@ def test_rows_without_a_label(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,F,C", [(32, 2047, 130), (9, 2060, 70), (31, 130, 1000), (33, 131, 1000), (8, 63, 4099), (4, 1, 65),
+                                   (17, 67, 64), (1, 2048, 30001)])
+def test_few_rows(V, F, C, dtype):
+    x, w, b, t, g = inputs(V, F, C, dtype, seed=V)
+    compare(x, w, b, t, g, "none")
+    compare(x, w, None, t, 1.0, "mean")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("F", [32, 29])
 @pytest.mark.parametrize("left", [math.nan, math.inf, 3e38])
