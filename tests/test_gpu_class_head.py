@@ -137,6 +137,14 @@ def test_loss_and_gradients(V, F, C, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,F,C", [(3000, 100, 4100), (700, 129, 13000), (2049, 264, 5000), (1025, 7, 6529)])
+def test_more_than_small_tiles_take(V, F, C, dtype):
+    x, w, b, t, g = inputs(V, F, C, dtype)
+    compare(x, w, b, t, g, "none")
+    compare(x, w, None, t, 1.0, "sum")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V,F,C", [(16500, 8, 150), (20000, 16, 8500), (16390, 40, 8200)])
 def test_blocks_of_rows_and_pieces_of_classes(V, F, C, dtype):
     x, w, b, t, g = inputs(V, F, C, dtype)
