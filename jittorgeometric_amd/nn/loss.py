@@ -140,7 +140,8 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
     does not matter.
 
     Products are summed in float32.  float32 entries keep 24 bits down to 2^-17 of the largest of
-    their array and 2^-39 of that largest below; an infinity or a NaN makes the logits it enters NaN.
+    their array and 2^-39 of that largest below; an infinity or a NaN makes the logits it enters NaN or
+    infinite.
     The gradient of the logits is rounded to bfloat16 on its way into the other gradients, or, in
     float32, held to 24 bits and at least 2^-40.  The scratch memory of a backward pass is up to a
     gigabyte of those, float32 sums of the size of weight, and one or two copies of x."""
