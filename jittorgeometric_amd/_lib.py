@@ -3,6 +3,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libjgamd.so")
@@ -140,8 +141,13 @@ def check_int32(who, *tensors):
 
 
 def needs_grad(*tensors):
-    """Whether a call with these inputs is recorded for a backward pass."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call with these inputs has to go through its autograd function: it is recorded for a
+    backward pass, or an input carries a tangent, which the function refuses and a direct call would lose."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    if getattr(forward_ad, "_current_level", 0) < 0:      # no dual level is open: nothing has a tangent
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # the current device's number without torch's checks around it, where this torch offers that
