@@ -19,6 +19,16 @@ int32_t launch_status(const char *what);
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Grid of `blocks` workgroups whose kernel numbers them by block_number().  A launch counts the threads
+// of a dimension in 32 bits and leaves out what is past them without an error (2^29 + 3 rows of 8
+// lanes: 24 threads ran), so that from 2^22 workgroups on they go on along y; the last row of the grid may
+// hold more than are asked for.
+inline dim3 grid_of_blocks(int64_t blocks)
+{
+    constexpr int64_t row = 1 << 22;
+    return blocks <= row ? dim3((unsigned)blocks) : dim3((unsigned)row, (unsigned)ceil_div(blocks, row));
+}
+
 // Bump allocator over the caller's workspace (256-byte granules).
 struct Carver {
     char *base;
@@ -109,6 +119,7 @@ __device__ __forceinline__ int wave_in_block()
 {
     return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 }
+__device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int bcast_i(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ float bcast_f(float v, int lane)

@@ -177,14 +177,14 @@ __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf
 
 template <int L> constexpr int norm_threads() { return L > 256 ? L : 256; }
 
-// L lanes a row, C vectors a lane; grid: rows / (threads / L)
+// L lanes a row, C vectors a lane; grid: rows / (threads / L) workgroups by block_number
 template <typename T, int L, int C, bool WHOLE>
 __global__ __launch_bounds__(norm_threads<L>()) void norm_fwd(NormArgs a)
 {
     constexpr int V = kVec<T>;
     __shared__ float scratch[2 * norm_threads<L>() / kWave];
     const int lane = threadIdx.x % L;
-    const int64_t row = (int64_t)blockIdx.x * (norm_threads<L>() / L) + threadIdx.x / L;
+    const int64_t row = block_number() * (norm_threads<L>() / L) + threadIdx.x / L;
     const bool mine = row < a.R;      // rows past the last are computed from nothing and not stored
     const int64_t base = row * a.F;
     const T *x = static_cast<const T *>(a.x), *y = static_cast<const T *>(a.y), *gate = static_cast<const T *>(a.gate);
@@ -531,7 +531,7 @@ JG_EXPORT int32_t jgamd_residual_norm_fwd(const void *x, const void *y, const vo
     auto launch = [&](auto type, auto l, auto c) {
         using T = decltype(type);
         constexpr int L = decltype(l)::value, C = decltype(c)::value, threads = norm_threads<L>();
-        const dim3 grid((unsigned)ceil_div(R, threads / L));
+        const dim3 grid = grid_of_blocks(ceil_div(R, threads / L));
         if (F % kVec<T> == 0) hipLaunchKernelGGL((norm_fwd<T, L, C, true>), grid, dim3(threads), 0, st, a);
         else hipLaunchKernelGGL((norm_fwd<T, L, C, false>), grid, dim3(threads), 0, st, a);
     };
