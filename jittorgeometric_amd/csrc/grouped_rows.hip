@@ -133,13 +133,14 @@ struct GroupedArgs {
     int whole;      // four neighbouring results always lie on an address that one store can take
 };
 
-// Workgroup blockIdx.x's place among `each` workgroups that read the same rows: group and place in it.  The
+// This workgroup's place among `each` workgroups that read the same rows: group and place in it.  The
 // groups go round the XCDs (every eighth workgroup runs on one), a group stays on one, one L2.  169343 rows,
 // 129 -> 200 floats, forward, dx and dW: 124, 140, 154 us with neighbours on different XCDs, 120, 128, 143 like this.
 __device__ __forceinline__ void group_of(int each, int *group, int *place)
 {
-    const int i = blockIdx.x / 8;
-    *group = i / each * 8 + blockIdx.x % 8;
+    const int64_t b = block_number();
+    const int i = (int)(b / 8);
+    *group = i / each * 8 + (int)(b % 8);
     *place = i % each;
 }
 static int64_t grid_of_groups(int64_t groups, int64_t each) { return ceil_div(groups, 8) * 8 * each; }
@@ -606,7 +607,7 @@ template <typename T, typename S, Layout WL> static int32_t launch_rows(const Gr
     const int64_t mtiles = (int64_t)a.M / S::BM + std::min<int64_t>(a.G, a.M) + 2;
     const int64_t blocks = grid_of_groups(mtiles, ceil_div(a.N, S::BN));
     if (blocks > 0x7fffffffLL) return fail(JGAMD_ERR_SIZE, "grouped_rows: M=%d N=%d G=%d is too large", a.M, a.N, a.G);
-    hipLaunchKernelGGL((grouped_rows<T, S, WL>), dim3((unsigned)blocks), dim3(S::kThreads), 0, s, a);
+    hipLaunchKernelGGL((grouped_rows<T, S, WL>), grid_of_blocks(blocks), dim3(S::kThreads), 0, s, a);
     return launch_status("grouped_rows");
 }
 
@@ -695,7 +696,7 @@ template <typename T, int BN, int BM> static int64_t launch_grad(const GradArgs 
     using S = Shape<T, BN, BM, 2, 2>;
     const int64_t tiles = grid_of_groups(pieces, ceil_div(a.N, BN) * ceil_div(a.K, BM));
     if (tiles <= 0x3fffffffLL)
-        hipLaunchKernelGGL((grouped_weight_grad<T, S>), dim3((unsigned)tiles), dim3(S::kThreads), 0, s, a);
+        hipLaunchKernelGGL((grouped_weight_grad<T, S>), grid_of_blocks(tiles), dim3(S::kThreads), 0, s, a);
     return tiles;
 }
 
