@@ -391,7 +391,7 @@ int32_t jgamd_dense_rows(const float *x1, const float *w1, int32_t K1, const flo
  * Softmax cross entropy of z = x w^T + bias without the [V][C] logits:
  *   lse[i]  = log sum_c exp(z[i,c])
  *   loss[i] = lse[i] - z[i,label[i]], 0 for labels outside [0,C)
- * x [V][F], w [C][F] (a row per class), bias [C] or NULL, all of `dtype`
+ * x [V][F] (V at most 2^31 - 256), w [C][F] (a row per class), bias [C] or NULL, all of `dtype`
  * (JGAMD_F32 / JGAMD_BF16; JGAMD_F32 = 0, JGAMD_BF16 = 1 below); sums, lse and
  * loss fp32.  `reduction`: JGAMD_LOSS_MEAN over the rows with a label (NaN when
  * there is none) and JGAMD_LOSS_SUM write loss[0] and count[0] = those rows,

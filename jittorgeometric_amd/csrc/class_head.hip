@@ -179,7 +179,7 @@ struct Copies {
     Copy of[2];
     const int32_t *y32;
     const int64_t *y64;
-    int blocks0;             // workgroups of the first; the others have the second
+    int blocks0, blocks;     // workgroups of the first; of both: the others have the second
     int F, ld, C;
 };
 
@@ -223,12 +223,14 @@ __global__ __launch_bounds__(256) void head_largest(Copies a)
     if (threadIdx.x == 0) c.largest[block] = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
 }
 
-// grid: x = blocks0 + the second array's, 256 pieces of 8 each
+// grid: blocks0 + the second array's workgroups by block_number, 256 pieces of 8 each
 template <typename T> __global__ __launch_bounds__(256) void head_parts(Copies a)
 {
-    const bool second = (int)blockIdx.x >= a.blocks0;
+    const int64_t number = block_number();
+    if (number >= a.blocks) return;
+    const bool second = number >= a.blocks0;
     const Copy &c = a.of[second];
-    const int block = second ? blockIdx.x - a.blocks0 : blockIdx.x;
+    const int block = (int)number - (second ? a.blocks0 : 0);
     float up = 1.f;
     if constexpr (sizeof(T) == 4) {      // the exponent, by every workgroup for itself
         static_assert(kMaxBlocks == 256, "a thread looks at one");
@@ -919,7 +921,8 @@ static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int3
 {
     if (V < 0 || F <= 0 || C <= 0)
         return fail(JGAMD_ERR_SIZE, "%s: V=%lld F=%d C=%d (V >= 0, the others positive)", who, (long long)V, F, C);
-    if (V > 0x7fffffffLL || F > kHeadMaxFeatures || C > 0x7fffff00)
+    // V: blocks of 256 rows, 512 threads each, stay under 2^32 threads
+    if (V > 0x7fffff00LL || F > kHeadMaxFeatures || C > 0x7fffff00)
         return fail(JGAMD_ERR_SIZE, "%s: V=%lld F=%d C=%d is too large", who, (long long)V, F, C);
     if (dtype != JGAMD_F32 && dtype != JGAMD_BF16) return fail(JGAMD_ERR_UNSUPPORTED, "%s: unknown dtype %d", who, dtype);
     if (reduction < 0 || reduction > JGAMD_LOSS_SUM) return fail(JGAMD_ERR_SIZE, "%s: unknown reduction %d", who, reduction);
@@ -929,7 +932,7 @@ static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int3
 template <typename T>
 static void head_copies(const Copy *of, int n, const HeadArgs &h, int number, uint32_t *largest, hipStream_t s)
 {
-    Copies a{{of[0], of[n - 1]}, h.y32, h.y64, 0, h.F, h.ld, h.C};
+    Copies a{{of[0], of[n - 1]}, h.y32, h.y64, 0, 0, h.F, h.ld, h.C};
     int64_t blocks = 0;
     for (int i = 0; i < n; i++) {
         a.of[i].largest = largest + (number + i) * kMaxBlocks;
@@ -938,8 +941,9 @@ static void head_copies(const Copy *of, int n, const HeadArgs &h, int number, ui
         blocks += ceil_div(of[i].R * (h.ld / 8), 256);
     }
     if (n == 1) a.blocks0 = (int)blocks;
+    a.blocks = (int)blocks;
     if (sizeof(T) == 4) hipLaunchKernelGGL(head_largest, dim3(n * kMaxBlocks), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((head_parts<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((head_parts<T>), grid_of_blocks(blocks), dim3(256), 0, s, a);
 }
 
 // x and w as parts: copies into the workspace, or the arrays themselves
