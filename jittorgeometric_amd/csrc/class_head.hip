@@ -615,8 +615,13 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
                     float d[8];
                     // z - l is taken before the scaling: both may be large
 #pragma unroll
-                    for (int r = 0; r < 8; r++)
-                        d[r] = __builtin_amdgcn_exp2f(fmaf(acc[i + r / 4][j][r % 4] - l, kLog2e, kUp));
+                    for (int r = 0; r < 8; r++) {
+                        float t = acc[i + r / 4][j][r % 4] - l;
+                        // bfloat16: the z of the statistics to the bit, so z <= l.  The z of a few rows of floats was
+                        // summed in another order, which shows where logits have no bits behind the point (4e6: t = 2)
+                        if (S::kParts > 1) t = t > 0.f ? 0.f : t;      // NaN stays
+                        d[r] = __builtin_amdgcn_exp2f(fmaf(t, kLog2e, kUp));
+                    }
                     if (at >= n && at < n + 8) {
 #pragma unroll
                         for (int r = 0; r < 8; r++)
