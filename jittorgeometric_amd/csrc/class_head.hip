@@ -6,17 +6,19 @@
 //     dx[i] = g[i] d[i] w,   dw = d^T (g x),   db = sum_i g[i] d[i]
 //
 // Forward: a workgroup keeps BM rows and walks a range of class tiles.  A lane holds four
-// consecutive classes of one row, so the running maximum and sum of exponentials of a row are two
-// registers of a lane; lanes, wavefronts and ranges are joined at the end, in a fixed order.
+// consecutive classes of one row in a fragment (32 of a tile of 256 x 256, in eights), so the running maximum
+// and sum of exponentials of a row are two registers of a lane; lanes, wavefronts and ranges are joined at the
+// end, in a fixed order.
 //
 // Backward: z is computed again, tile by tile, and d is written for a block of rows and a piece of
 // the classes (at most kPieceBytes, in the type of x); two products take it from there.
 // dx sums over the pieces and dw over the blocks of rows in fp32 (a workspace where several take
 // part), rounded once at the end.  Four products instead of the three of a loss that keeps its
-// logits.  d in bfloat16 is off by 2^-9 of itself, like any gradient of logits of that type; it is kept
+// logits.  d in bfloat16 is off by 2^-8 of itself, like any gradient of logits of that type; it is kept
 // without g, since -1 is exact but g (1 / rows) rounded once for all rows would shift every result alike
 // (16384 rows of 131072 classes: dw off by 3.1e-3 with g in d, 1.7e-3 without).  g multiplies the fp32
-// sums where it is one number, and dx's rows and a copy of x where it is one a row.
+// sums where it is one number, and dx's rows and a copy of x where it is one a row (rounded to bfloat16 once
+// more there: its roundings are as many as the entries and independent of each other).
 //
 // Bound by the matrix units from some hundred rows on, by reading w below that.
 #include <algorithm>
@@ -27,24 +29,25 @@
 namespace jg {
 
 constexpr int kHeadMaxFeatures = 1 << 20;
-constexpr int64_t kPieceBytes = (int64_t)1 << 30;      // of d.  16384 rows, 512 features, 131072 classes, bfloat16: 9.7 ms with pieces of 512 MB, 9.4 with 1 GB
+// of d.  16384 rows, 512 features, 131072 classes, bfloat16: 9.7 ms with pieces of 512 MB, 9.4 with 1 GB
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 constexpr int kBlockRows = 16384;      // rows of a block of the backward pass
 constexpr int kJoinThreads = 256;
 constexpr int kCus = 256;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kPad = 128;      // classes between the rows of d: rows a power of two apart meet in one channel of the L2
 
-// 256 x 256 results, eight wavefronts of 128 x 64, two stages of 64 KB: steps of 64, or of 32 for floats in
-// two parts.  Two workgroups a compute unit, one of which could multiply while the other takes exponentials,
-// need narrower tiles and steps of 32, whose loads ask for 64 bytes of a row.  The statistics of 16384 rows,
-// 512 features, 131072 classes in bfloat16: 2.43 ms; 256 x 256 with four stages of 32: 2.61; two workgroups of
-// 256 x 128: 2.77, of 128 x 256: 2.52.
+// 256 x 256 results, eight wavefronts of 128 x 64, two stages of 64 KB: steps of 64.  Two workgroups a compute
+// unit, one of which could multiply while the other takes exponentials, need narrower tiles and steps of 32,
+// whose loads ask for 64 bytes of a row.  The statistics of 16384 rows, 512 features, 131072 classes in
+// bfloat16: 2.43 ms; 256 x 256 with four stages of 32: 2.61; two workgroups of 256 x 128: 2.77, of 128 x 256:
+// 2.52.  Floats in three parts: 256 x 128, two stages of 72 KB, steps of 32.
 template <typename T> struct HeadShapeOf;
 template <> struct HeadShapeOf<bf16> {
     using S = StreamShape<1, 256, 256, 2, 4, 64, 2>;
 };
 template <> struct HeadShapeOf<float> {
-    using S = StreamShape<2, 256, 256, 2, 4, 32, 2>;
+    using S = StreamShape<3, 256, 128, 4, 2, 32, 2>;
 };
 template <typename T> using HeadShape = typename HeadShapeOf<T>::S;
 // tiles of a few rows, two workgroups a compute unit
@@ -53,22 +56,17 @@ template <> struct HeadFewOf<bf16> {
     using S = StreamShape<1, 128, 32, 4, 1, 64, 4>;
 };
 template <> struct HeadFewOf<float> {
-    using S = StreamShape<2, 128, 64, 4, 1, 32, 3>;
+    using S = StreamShape<3, 128, 64, 4, 1, 32, 2>;
 };
 template <typename T> using HeadFew = typename HeadFewOf<T>::S;
 
-// Floats enter as two float16 parts: a 2^e = a1 + a2, each the remainder rounded to 11 bits, which is
-// all of a's 24 bits but the last; e brings the array's largest entry to 2^14 .. 2^15.  Dropping a2 b2
-// (under 2^-24 of a b) leaves three products, half of what three bfloat16 parts take.  float16 ends at
-// 2^-24: an entry under 2^-17 of the array's largest keeps an absolute precision of 2^-39 of that largest
-// instead of 24 bits of its own: the logits of every row are off by 2^-39 of what the largest entry gives,
-// which is nothing to a softmax unless that row's own logits reach 10^5.  d is stored times 2^15 (|d| <= 1): probabilities under 2^-17 keep 2^-40.
-constexpr int kDExponent = 15;
-constexpr int kMaxBlocks = 256;      // workgroups that look for an array's largest entry
-
+// Floats enter as the three bfloat16 parts of tile_product.h, six products of them: every entry keeps its own
+// 24 bits, and so does every entry of d, whatever the others of its row, its class or its array are.  Two
+// float16 parts under one exponent an array take half the products (4099 rows, 256 features, 32003 classes,
+// training: 1.05 instead of 1.61 ms) and lose them: a row 1e8 times the others moved the others' losses by 1e-3,
+// and the gradients of classes of probability 1e-12 were off by 0.4 of themselves.
 struct HeadArgs {
     const bf16 *x, *w;           // [V][ld], [C][ld] as parts (stream_product.h)
-    const int *exponents;        // e of x, w, g x where they are split, else NULL
     int64_t part_x, part_w;
     int ld;                      // F rounded up to 8
     const void *bias;            // [C] of T, or NULL
@@ -85,9 +83,6 @@ __device__ __forceinline__ int64_t label_in(const int32_t *y32, const int64_t *y
     return y >= 0 && y < C ? y : -1;
 }
 __device__ __forceinline__ int64_t head_label(const HeadArgs &a, int64_t row) { return label_in(a.y32, a.y64, a.C, row); }
-
-// 2^-(e1 + e2), as near as a float comes: logits that need more are under 2^-80, or infinite
-__device__ __forceinline__ float unscale(int e1, int e2) { return ldexpf(1.f, min(max(-(e1 + e2), -126), 127)); }
 
 // (m, s): s exponentials relative to m.  An m of -inf holds nothing (s = 0).
 __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s2)
@@ -133,17 +128,10 @@ __device__ __forceinline__ int tiles_of(int mtiles, int ntiles)
     return first < all ? (int)((all - 1 - first) / g + 1) : 0;
 }
 
-// two floats as two float16 in one register, rounded to nearest even
-__device__ __forceinline__ uint32_t pack_half(float a, float b)
-{
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    const f16x2 v = {(_Float16)a, (_Float16)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
-__device__ __forceinline__ float half_lo(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)v); }
-__device__ __forceinline__ float half_hi(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16)); }
+// the largest finite bfloat16
+constexpr float kBf16Max = 0x1.fep+127f;
 
-// eight neighbouring values as one bfloat16 or two float16 parts, kept where `keep` has ones
+// eight neighbouring values as one or three bfloat16 parts, kept where `keep` has ones
 template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int64_t part, float (&v)[8], uint32_t keep)
 {
 #pragma unroll
@@ -151,10 +139,10 @@ template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int
         u32x4 w;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            w[i] = PARTS == 1 ? pack_bf16(v[2 * i], v[2 * i + 1]) : pack_half(v[2 * i], v[2 * i + 1]);
+            w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
             if (s + 1 < PARTS) {
-                v[2 * i] -= half_lo(w[i]);
-                v[2 * i + 1] -= half_hi(w[i]);
+                v[2 * i] -= bf16_lo(w[i]);
+                v[2 * i + 1] -= bf16_hi(w[i]);
             }
             w[i] &= keep;
         }
@@ -164,7 +152,7 @@ template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int
 
 // One array to be laid out as parts: [R][F] of T to [R][ld], zero behind F; rows times scale[R] unless
 // that is NULL (a row times zero is zero whatever it holds), or, with `labelled`, zero without a label:
-// what a padded row holds neither enters dW as 0 x NaN nor sets the array's exponent.
+// what a padded row holds does not enter dW as 0 x NaN.
 struct Copy {
     const void *src;
     const float *scale;
@@ -172,8 +160,6 @@ struct Copy {
     int64_t R;
     bf16 *dst;
     int64_t part;            // elements between the parts
-    uint32_t *largest;       // [kMaxBlocks]: bits of the largest finite |entry| each workgroup saw
-    int *exponent;
 };
 struct Copies {
     Copy of[2];
@@ -198,31 +184,6 @@ template <typename T> __device__ __forceinline__ Eight<T> copy_piece(const Copie
     return e;
 }
 
-// grid: x = kMaxBlocks for each of the arrays
-__global__ __launch_bounds__(256) void head_largest(Copies a)
-{
-    __shared__ uint32_t s_top[4];
-    const Copy &c = a.of[blockIdx.x >= (unsigned)kMaxBlocks];
-    const int block = blockIdx.x % kMaxBlocks;
-    const int64_t pieces = c.R * (a.ld / 8);
-    uint32_t top = 0;
-    auto see = [&](float v) {
-        const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
-        top = max(top, bits < 0x7f800000u ? bits : 0u);
-    };
-#pragma unroll 4
-    for (int64_t id = (int64_t)block * 256 + threadIdx.x; id < pieces; id += kMaxBlocks * 256) {
-        const Eight<float> e = copy_piece<float>(a, c, id);
-#pragma unroll
-        for (int i = 0; i < 4; i++) see(e.a[i]), see(e.b[i]);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
-    if (lane_id() == 0) s_top[wave_in_block()] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) c.largest[block] = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-}
-
 // grid: blocks0 + the second array's workgroups by block_number, 256 pieces of 8 each
 template <typename T> __global__ __launch_bounds__(256) void head_parts(Copies a)
 {
@@ -230,29 +191,28 @@ template <typename T> __global__ __launch_bounds__(256) void head_parts(Copies a
     if (number >= a.blocks) return;
     const bool second = number >= a.blocks0;
     const Copy &c = a.of[second];
-    const int block = (int)number - (second ? a.blocks0 : 0);
-    float up = 1.f;
-    if constexpr (sizeof(T) == 4) {      // the exponent, by every workgroup for itself
-        static_assert(kMaxBlocks == 256, "a thread looks at one");
-        __shared__ uint32_t s_top[4];
-        uint32_t top = c.largest[threadIdx.x];
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
-        if (lane_id() == 0) s_top[wave_in_block()] = top;
-        __syncthreads();
-        top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-        const int e = top == 0 ? 0 : min(14 - ((int)(top >> 23) - 127), 126);      // a subnormal counts as 2^-127
-        up = ldexpf(1.f, e);
-        if (block == 0 && threadIdx.x == 0) *c.exponent = e;
-    }
-    const int64_t id = (int64_t)block * 256 + threadIdx.x;
+    const int64_t id = (number - (second ? a.blocks0 : 0)) * 256 + threadIdx.x;
     if (id >= c.R * (a.ld / 8)) return;
     const Eight<T> e = copy_piece<T>(a, c, id);
     if constexpr (sizeof(T) == 4) {
-        float v[8];
+        // the first part stays finite: past kBf16Max the second takes what is left.  An infinity gives
+        // infinity and NaN as the other two, a NaN (which the clamp makes a number) NaN.
+        float first[8], rest[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = e.a[i] * up, v[4 + i] = e.b[i] * up;
-        store_parts8<2>(c.dst + id * 8, c.part, v, 0xffffffffu);
+        for (int i = 0; i < 8; i++) {
+            const float v = i < 4 ? e.a[i & 3] : e.b[i & 3];
+            first[i] = fminf(fmaxf(v, -kBf16Max), kBf16Max);
+            rest[i] = v;
+        }
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            w[i] = pack_bf16(first[2 * i], first[2 * i + 1]);
+            rest[2 * i] -= bf16_lo(w[i]);
+            rest[2 * i + 1] -= bf16_hi(w[i]);
+        }
+        *reinterpret_cast<u32x4 *>(c.dst + id * 8) = w;
+        store_parts8<2>(c.dst + id * 8 + c.part, c.part, rest, 0xffffffffu);
     } else *reinterpret_cast<u32x4 *>(c.dst + id * 8) = e.v;
 }
 
@@ -260,15 +220,12 @@ template <typename T> __global__ __launch_bounds__(256) void head_parts(Copies a
 template <typename T, typename Product, typename S>
 __device__ __forceinline__ void logits(f32x4 (&acc)[S::FN][S::FM], const HeadArgs &h, int c0)
 {
-    if (S::kParts == 1 && !h.bias) return;
-    const float down = S::kParts == 2 ? unscale(h.exponents[0], h.exponents[1]) : 1.f;
+    if (!h.bias) return;
 #pragma unroll
     for (int i = 0; i < S::FN; i++) {
         const f32x4 b = bias4<T>(h.bias, c0 + Product::n_of(i), h.C);
 #pragma unroll
-        for (int j = 0; j < S::FM; j++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) acc[i][j][r] = S::kParts == 2 ? fmaf(acc[i][j][r], down, b[r]) : acc[i][j][r] + b[r];
+        for (int j = 0; j < S::FM; j++) acc[i][j] += b;
     }
 }
 
@@ -365,9 +322,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void head_stats(HeadArgs a, int ran
 // being laid out as parts for it.  kThinRows rows of x stand in LDS; sixteen lanes share four classes, 4 k a lane
 // and step.  The 32 sums of a group meet in a transposing reduction (16 + 8 + 4 + 2 shuffles) that leaves each
 // lane one class of two rows, whose running maximum and sum it keeps.  Bound by reading w for up to kThinRows
-// rows, by the vector unit beyond.  Whole calls, with parts and like this: 4 rows, 387 features, 48749 classes 79
-// and 25 us; 256 features, 50021 classes: 7 rows 46 and 22, 24 rows 47 and 43, 32 rows 47 and 43; 2000 features,
-// 20000 classes, 32 rows: 175 and 156.  (bfloat16 of odd widths, copied once: 8 rows 23 and 27, 32 rows 23 and 46.)
+// rows, by the vector unit beyond.  Whole calls, with parts and like this: 4 rows, 387 features, 48749 classes 66
+// and 26 us; 256 features, 50021 classes: 7 rows 48 and 24, 24 rows 47 and 45, 32 rows 48 and 46, 48 rows 49 and 65;
+// 2000 features, 20000 classes, 32 rows: 193 and 157.  (bfloat16 of odd widths, copied once: 8 rows 23 and 27, 32 rows 23 and 46.)
 // grid: x = blocks of kThinRows rows x ranges of tiles of 64 classes
 constexpr int kThinRows = 8;
 constexpr int kThinMost = 32;            // rows of a call, at most
@@ -597,7 +554,6 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
             int m0, n0;
             corner(t, &m0, &n0);
             logits<T, Product, S>(acc, h, a.c0 + n0);
-            constexpr float kUp = S::kParts == 2 ? kDExponent : 0, kOne = S::kParts == 2 ? 1 << kDExponent : 1;
             const bool edge = n0 + S::BN > a.classes;
 #pragma unroll
             for (int j = 0; j < S::FM; j++) {
@@ -613,19 +569,18 @@ template <typename T, typename S> __global__ __launch_bounds__(S::kThreads, 2) v
                 for (int i = 0; i < S::FN; i += 2) {
                     const int n = Product::n_of(i);
                     float d[8];
-                    // z - l is taken before the scaling: both may be large
 #pragma unroll
                     for (int r = 0; r < 8; r++) {
                         float t = acc[i + r / 4][j][r % 4] - l;
                         // bfloat16: the z of the statistics to the bit, so z <= l.  The z of a few rows of floats was
                         // summed in another order, which shows where logits have no bits behind the point (4e6: t = 2)
                         if (S::kParts > 1) t = t > 0.f ? 0.f : t;      // NaN stays
-                        d[r] = __builtin_amdgcn_exp2f(fmaf(t, kLog2e, kUp));
+                        d[r] = __builtin_amdgcn_exp2f(t * kLog2e);
                     }
                     if (at >= n && at < n + 8) {
 #pragma unroll
                         for (int r = 0; r < 8; r++)
-                            if (n + r == at) d[r] -= kOne;
+                            if (n + r == at) d[r] -= 1.f;
                     }
                     if (edge) {
                         if (n0 + n >= a.ld) continue;
@@ -650,7 +605,6 @@ struct SumArgs {
     float *acc, *part;  // [M][N], [splits][M][N]
     void *out_b;        // sums of Q over k, [M]; the same three arrays for them, NULL: not wanted
     float *acc_b, *part_b;
-    const int *exponent_p;       // e of P where the operands are split (those of Q: kDExponent), else NULL
     const float *row_scale;      // g of m, or NULL:
     const float *grad;           // g = grad[0] (/ count[0]); both NULL: 1
     const int32_t *count;
@@ -658,23 +612,17 @@ struct SumArgs {
     int whole;          // four neighbouring values lie on an address that one access can take
 };
 
-// what a sum is multiplied by: 2^down, which alone may be no float, then g
-struct SumScale {
-    int down;
-    float g;
-    __device__ __forceinline__ float of(float v) const { return ldexpf(v, down) * g; }
-};
-__device__ __forceinline__ SumScale sum_scale(const SumArgs &a, int m, bool sum_of_q)
+// what a sum is multiplied by
+__device__ __forceinline__ float sum_scale(const SumArgs &a, int m)
 {
-    const int down = a.exponent_p ? -kDExponent - (sum_of_q ? 0 : *a.exponent_p) : 0;
-    if (a.row_scale) return {down, a.row_scale[m]};
-    if (!a.grad) return {down, 1.f};
-    if (!a.count) return {down, a.grad[0]};
-    return {down, a.count[0] > 0 ? a.grad[0] / (float)a.count[0] : 0.f};      // no row counts: every sum is zero
+    if (a.row_scale) return a.row_scale[m];
+    if (!a.grad) return 1.f;
+    if (!a.count) return a.grad[0];
+    return a.count[0] > 0 ? a.grad[0] / (float)a.count[0] : 0.f;      // no row counts: every sum is zero
 }
 
 template <typename T>
-__device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc, int64_t at, f32x4 v, int n, const SumScale &scale)
+__device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc, int64_t at, f32x4 v, int n, float g)
 {
     if (!a.first) {
         if (a.whole && n >= 4) v += *reinterpret_cast<const f32x4 *>(acc + at);
@@ -684,7 +632,7 @@ __device__ __forceinline__ void finish4(const SumArgs &a, void *out, float *acc,
                 if (r < n) v[r] += acc[at + r];
         }
     }
-    if (a.last) store4<T>(static_cast<T *>(out) + at, f32x4{scale.of(v[0]), scale.of(v[1]), scale.of(v[2]), scale.of(v[3])}, n, a.whole);
+    if (a.last) store4<T>(static_cast<T *>(out) + at, v * g, n, a.whole);
     else store4<float>(acc + at, v, n, a.whole);
 }
 
@@ -721,10 +669,10 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
             for (int j = 0; j < S::FM; j++) {
                 const int m = m0 + Product::m_of(j);
                 if (m >= a.M) continue;
-                const SumScale scale = a.splits > 1 ? SumScale{0, 1.f} : sum_scale(a, m, false);
+                const float g = a.splits > 1 ? 1.f : sum_scale(a, m);
                 if (SUMS == kSumQ && n0 == 0 && Product::n_of(0) == 0) {
                     if (a.splits > 1) a.part_b[(int64_t)split * a.M + m] = sums[j][0];
-                    else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1, sum_scale(a, m, true));
+                    else finish4<T>(a, a.out_b, a.acc_b, m, sums[j], 1, g);
                 }
 #pragma unroll
                 for (int i = 0; i < S::FN; i++) {
@@ -732,7 +680,7 @@ template <typename T, typename S, Layout QL, Sums SUMS> __global__ __launch_boun
                     if (n >= a.N) continue;
                     const int64_t at = (int64_t)m * a.N + n;
                     if (a.splits > 1) store4<float>(a.part + (int64_t)split * a.M * a.N + at, acc[i][j], a.N - n, a.whole);
-                    else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n, scale);
+                    else finish4<T>(a, a.out, a.acc, at, acc[i][j], a.N - n, g);
                 }
             }
         });
@@ -751,7 +699,7 @@ template <typename T> __global__ __launch_bounds__(256) void head_join(SumArgs a
 #pragma unroll 8
     for (int k = 0; k < a.splits; k++) v += part[k * stride];
     if (a.last)
-        static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(sum_scale(a, a.row_scale ? (int)(at / a.N) : 0, b).of(v));
+        static_cast<T *>(b ? a.out_b : a.out)[at] = from_float<T>(v * sum_scale(a, a.row_scale ? (int)(at / a.N) : 0));
     else acc[at] = v;
 }
 
@@ -775,14 +723,14 @@ __global__ __launch_bounds__(256) void head_bias(const bf16 *__restrict__ d, int
     if (c < classes) {      // ld is a multiple of 8 and holds zeros behind the last class
 #pragma unroll 4
         for (int m = strand; m < rows; m += 32) {
-            const float g = sizeof(T) == 2 ? scale[m] : scale[m] / (1 << kDExponent);
+            const float g = scale[m];
 #pragma unroll
             for (int s = 0; s < HeadShape<T>::kParts; s++) {
                 const u32x4 w = *reinterpret_cast<const u32x4 *>(d + s * part + (int64_t)m * ld + c);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    v[2 * i] = fmaf(g, sizeof(T) == 2 ? bf16_lo(w[i]) : half_lo(w[i]), v[2 * i]);
-                    v[2 * i + 1] = fmaf(g, sizeof(T) == 2 ? bf16_hi(w[i]) : half_hi(w[i]), v[2 * i + 1]);
+                    v[2 * i] = fmaf(g, bf16_lo(w[i]), v[2 * i]);
+                    v[2 * i + 1] = fmaf(g, bf16_hi(w[i]), v[2 * i + 1]);
                 }
             }
         }
@@ -814,9 +762,10 @@ template <typename T> static bool head_thin_takes(int64_t V, int F)
 {
     return sizeof(T) == 4 && V <= kThinMost && F <= kThinFeatures;
 }
-// Small tiles for the logits where large ones would leave half of the chip without one.  Forward, floats and
-// bfloat16: 100 rows, 1000 features, 16000 classes, 63 tiles: 116 and 41 us, 70 and 28 in small ones; 2000 rows,
-// 256, 4000, 128 tiles: 42 and 22, 35 and 18; 200 rows, 200, 40000, 157 tiles: 52 and 21, 60 and 28.
+// Small tiles for the logits where large ones would leave half of the chip without one.  Forward, large and small:
+// floats, 100 rows, 1000 features, 16000 classes, 63 tiles: 112 and 77 us; 500, 256, 2000, 32 tiles: 34 and 22;
+// 300, 256, 16000, 189 tiles: 42 and 49.  bfloat16, 100, 1000, 16000: 41 and 28; 2000, 256, 4000, 128 tiles: 22
+// and 18; 200, 200, 40000, 157 tiles: 21 and 28.
 template <typename T> static bool head_few(int64_t V, int C)
 {
     return V <= HeadFew<T>::BM || ceil_div(V, HeadShape<T>::BM) * ceil_div(C, HeadShape<T>::BN) <= kCus / 2;
@@ -885,7 +834,7 @@ template <typename T> static size_t parts_elements(int64_t R, int F)
 
 template <typename T> struct HeadScratch {      // of the forward pass, then of the backward pass
     size_t x = 0, w = 0, gx = 0;                                      // bfloat16
-    size_t largest = 0, scale = 0;                                    // uint32_t (and the exponents), float
+    size_t scale = 0;                                                 // float
     size_t stats = 0, at_label = 0, blocks = 0;                       // float2, float, double + int
     size_t d = 0;                                                     // bfloat16
     size_t part = 0, part_b = 0, acc_x = 0, acc_w = 0, acc_b = 0;     // float
@@ -894,7 +843,6 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
         if (backward || !head_thin_takes<T>(V, F)) {
             x = parts_elements<T>(V, F);
             w = parts_elements<T>(C, F);
-            largest = sizeof(T) == 4 ? 3 * kMaxBlocks + 3 : 0;
         }
         if (!backward) {
             stats = (size_t)head_ranges<T>(V, F, C) * V;
@@ -915,8 +863,7 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
     }
     size_t bytes() const
     {
-        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(gx, 2) + carve_bytes(largest, 4) +
-               carve_bytes(scale, 4) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
+        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(gx, 2) + carve_bytes(scale, 4) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
                carve_bytes(blocks, 8) + carve_bytes(blocks, 4) + carve_bytes(d, 2) + carve_bytes(part, 4) +
                carve_bytes(part_b, 4) + carve_bytes(acc_x, 4) + carve_bytes(acc_w, 4) + carve_bytes(acc_b, 4);
     }
@@ -933,32 +880,21 @@ static int32_t head_check(const char *who, int64_t V, int32_t F, int32_t C, int3
     if (reduction < 0 || reduction > JGAMD_LOSS_SUM) return fail(JGAMD_ERR_SIZE, "%s: unknown reduction %d", who, reduction);
     return 0;
 }
-// lays out one or two arrays as parts; `numbers`: the first one's place among the three that have exponents
-template <typename T>
-static void head_copies(const Copy *of, int n, const HeadArgs &h, int number, uint32_t *largest, hipStream_t s)
+// lays out one or two arrays as parts
+template <typename T> static void head_copies(const Copy *of, int n, const HeadArgs &h, hipStream_t s)
 {
-    Copies a{{of[0], of[n - 1]}, h.y32, h.y64, 0, 0, h.F, h.ld, h.C};
-    int64_t blocks = 0;
-    for (int i = 0; i < n; i++) {
-        a.of[i].largest = largest + (number + i) * kMaxBlocks;
-        a.of[i].exponent = reinterpret_cast<int *>(largest + 3 * kMaxBlocks) + number + i;
-        if (i == 1) a.blocks0 = (int)blocks;
-        blocks += ceil_div(of[i].R * (h.ld / 8), 256);
-    }
-    if (n == 1) a.blocks0 = (int)blocks;
-    a.blocks = (int)blocks;
-    if (sizeof(T) == 4) hipLaunchKernelGGL(head_largest, dim3(n * kMaxBlocks), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((head_parts<T>), grid_of_blocks(blocks), dim3(256), 0, s, a);
+    const int64_t first = ceil_div(of[0].R * (h.ld / 8), 256), second = n == 2 ? ceil_div(of[1].R * (h.ld / 8), 256) : 0;
+    const Copies a{{of[0], of[n - 1]}, h.y32, h.y64, (int)first, (int)(first + second), h.F, h.ld, h.C};
+    hipLaunchKernelGGL((head_parts<T>), grid_of_blocks(first + second), dim3(256), 0, s, a);
 }
 
 // x and w as parts: copies into the workspace, or the arrays themselves
 template <typename T>
-static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs, bf16 *ws, uint32_t *largest, hipStream_t s)
+static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs, bf16 *ws, hipStream_t s)
 {
     h->ld = (int)parts_ld(h->F);
     h->part_x = h->V * h->ld;
     h->part_w = (int64_t)h->C * h->ld;
-    h->exponents = sizeof(T) == 4 ? reinterpret_cast<const int *>(largest + 3 * kMaxBlocks) : nullptr;
     if (parts_in_place<T>(h->F)) {
         h->x = static_cast<const bf16 *>(x);
         h->w = static_cast<const bf16 *>(w);
@@ -968,9 +904,8 @@ static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs
     h->w = ws;
     const int64_t blocks = ceil_div(h->part_x / 8, 256) + ceil_div(h->part_w / 8, 256);
     if (blocks > 0x7fffffffLL) return fail(JGAMD_ERR_SIZE, "linear_cross_entropy: V=%lld F=%d C=%d is too large", (long long)h->V, h->F, h->C);
-    const Copy of[2] = {{x, nullptr, 1, h->V, xs, h->part_x, nullptr, nullptr},
-                        {w, nullptr, 0, h->C, ws, h->part_w, nullptr, nullptr}};
-    head_copies<T>(of, 2, *h, 0, largest, s);
+    const Copy of[2] = {{x, nullptr, 1, h->V, xs, h->part_x}, {w, nullptr, 0, h->C, ws, h->part_w}};
+    head_copies<T>(of, 2, *h, s);
     return launch_status("linear_cross_entropy");
 }
 
@@ -1012,7 +947,6 @@ static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t re
     const HeadScratch<T> n(h.V, h.F, h.C, false);
     Carver carve(ws);
     bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w);
-    uint32_t *largest = carve.take<uint32_t>(n.largest);
     float2 *stats = carve.take<float2>(n.stats);
     float *at_label = carve.take<float>(n.at_label);
     double *block_sum = carve.take<double>(n.blocks);
@@ -1023,7 +957,7 @@ static int32_t head_forward(HeadArgs h, const void *x, const void *w, int32_t re
         const int ranges = head_ranges<T>(h.V, h.F, h.C);
         const bool thin = head_thin_takes<T>(h.V, h.F);
         if (!thin)
-            if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, largest, st)) return rc;
+            if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
         if (thin) {
             const size_t lds = sizeof(float) * kThinRows * (size_t)(ceil_div(h.F, 64) * 64);
             raise_lds<&head_thin>(sizeof(float) * kThinRows * kThinFeatures);
@@ -1051,21 +985,20 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
     const HeadScratch<T> n(h.V, h.F, h.C, true);
     Carver carve(ws);
     bf16 *xs = carve.take<bf16>(n.x), *wp = carve.take<bf16>(n.w), *gx = carve.take<bf16>(n.gx);
-    uint32_t *largest = carve.take<uint32_t>(n.largest);
     float *scale = carve.take<float>(n.scale);
     bf16 *d = carve.take<bf16>(n.d);
     float *part = carve.take<float>(n.part), *part_b = carve.take<float>(n.part_b);
     float *acc_x = carve.take<float>(n.acc_x), *acc_w = carve.take<float>(n.acc_w), *acc_b = carve.take<float>(n.acc_b);
     if (h.V > 0)
-        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, largest, st)) return rc;
+        if (int32_t rc = head_operands<T>(&h, x, w, xs, wp, st)) return rc;
     if (h.V == 0) h.ld = (int)parts_ld(h.F);
     const bool per_row = reduction == JGAMD_LOSS_NONE;
     if (per_row && h.V > 0) hipLaunchKernelGGL(head_row_scale, dim3((unsigned)ceil_div(h.V, 256)), dim3(256), 0, st, h, grad, scale);
     // what dW sums: x, times one g a row if there is one, rows without a label zero (7 us of 9 ms for bf16)
     const bool own_copy = per_row || parts_in_place<T>(h.F);
     if (dw && own_copy && h.V > 0) {
-        const Copy of{x, per_row ? scale : nullptr, !per_row, h.V, gx, h.V * h.ld, nullptr, nullptr};
-        head_copies<T>(&of, 1, h, 2, largest, st);
+        const Copy of{x, per_row ? scale : nullptr, !per_row, h.V, gx, h.V * h.ld};
+        head_copies<T>(&of, 1, h, st);
     }
     const int ldd = (int)s.classes + kPad;
     const int64_t part_d = s.rows * ldd;
@@ -1087,7 +1020,6 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
             if (dx && rows > 0) {
                 a.row_scale = per_row ? scale + row0 : nullptr;
                 a.p = h.w + (int64_t)c0 * h.ld, a.part_p = h.part_w;
-                a.exponent_p = h.exponents ? h.exponents + 1 : nullptr;
                 a.M = rows, a.K = classes;
                 a.splits = sum_splits<T>(s.rows, h.F, s.classes);
                 a.k_split = (int)(ceil_div(ceil_div(s.classes, a.splits), 64) * 64);
@@ -1098,7 +1030,6 @@ static int32_t head_backward(HeadArgs h, const void *x, const void *w, const flo
             if (dw) {
                 a.p = (own_copy ? gx : h.x) + row0 * h.ld, a.part_p = own_copy ? h.V * h.ld : h.part_x;
                 a.row_scale = nullptr;
-                a.exponent_p = h.exponents ? h.exponents + (own_copy ? 2 : 0) : nullptr;
                 a.M = classes, a.K = rows;
                 a.splits = sum_splits<T>(s.classes, h.F, s.rows);
                 a.k_split = (int)(ceil_div(ceil_div(s.rows, a.splits), 64) * 64);

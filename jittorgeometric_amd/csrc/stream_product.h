@@ -1,6 +1,6 @@
-// The products of tile_product.h for operands that lie in memory as 16-bit parts on 16-byte addresses
-// (one bfloat16, or two float16 whose three products a1b1 + a1b2 + a2b1 stand for one of floats): tiles go from memory to LDS directly (buffer_load ... lds), several steps ahead, and a
-// workgroup that owns several tiles keeps loading across their borders.
+// The products of tile_product.h for operands that lie in memory as bfloat16 parts (one, or three for
+// floats) on 16-byte addresses: tiles go from memory to LDS directly (buffer_load ... lds), several steps
+// ahead, and a workgroup that owns several tiles keeps loading across their borders.
 //
 // A step is 32 or 64 values of k.  STAGES steps have room in LDS; while one is multiplied, the next
 // STAGES - 1 are loaded or on their way.  Per step a wavefront waits until its own loads of that step
@@ -39,7 +39,7 @@ struct StreamTile {
 
 template <int PARTS, int BN_, int BM_, int WN_, int WM_, int STEP_, int STAGES_> struct StreamShape {
     static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, kStep = STEP_, kStages = STAGES_, kParts = PARTS;
-    static_assert(PARTS == 1 || PARTS == 2, "one bfloat16 or two float16");
+    static_assert(PARTS == 1 || PARTS == 3, "of a bfloat16 or of a float");
     static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
     static constexpr int FN = BN / WN / 16, FM = BM / WM / 16;
     static constexpr int kLoadsP = BN * kStep / 512 / kWaves, kLoadsQ = BM * kStep / 512 / kWaves;      // of a wavefront, step and part
@@ -87,8 +87,11 @@ template <int PARTS, int WIDTH, int STEP> struct StreamOfWidth;
 template <int PARTS, int STEP> struct StreamOfWidth<PARTS, 256, STEP> {
     using S = StreamShape<PARTS, 256, 256, 2, 4, STEP, 2>;
 };
+template <int STEP> struct StreamOfWidth<3, 256, STEP> {      // 256 x 256 of three parts do not fit into LDS twice
+    using S = StreamShape<3, 256, 128, 4, 2, STEP, 2>;
+};
 template <int PARTS, int STEP> struct StreamOfWidth<PARTS, 128, STEP> {
-    using S = StreamShape<PARTS, 128, 256, 2, 4, STEP, 3>;
+    using S = StreamShape<PARTS, 128, 256, 2, 4, STEP, PARTS == 1 ? 3 : 2>;
 };
 template <int PARTS, int STEP> struct StreamOfWidth<PARTS, 64, STEP> {
     using S = StreamShape<PARTS, 64, 256, 1, 4, STEP, 2>;
@@ -187,13 +190,6 @@ template <typename S, Layout PL, Layout QL, bool PAIRS = PL == kAlongK> struct S
         __builtin_amdgcn_raw_buffer_store_b128(v, r, (int)(exists ? at : kStreamRange), 0, 0);
     }
 
-    __device__ __forceinline__ static f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c)
-    {
-        typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-        if constexpr (S::kParts == 2)
-            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
     // the products of fragments i0 .. i1 - 1 of P, parts from the smallest products to the largest
     template <int PARTS>
     __device__ __forceinline__ static void multiply(f32x4 (&acc)[S::FN][S::FM], const bf16x8 (&fp)[S::kParts][S::FN],
@@ -207,7 +203,7 @@ template <typename S, Layout PL, Layout QL, bool PAIRS = PL == kAlongK> struct S
                 for (int i = i0; i < i1; i++)
 #pragma unroll
                     for (int j = 0; j < S::FM; j++)
-                        acc[i][j] = mma(fp[a][i], fq[sum - a][j], acc[i][j]);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[a][i], fq[sum - a][j], acc[i][j], 0, 0, 0);
     }
 
     // Multiplies tiles 0 .. tiles - 1: tile(t) describes one (a StreamTile; cheap, called twice),
@@ -311,18 +307,21 @@ template <typename S, Layout PL, Layout QL, bool PAIRS = PL == kAlongK> struct S
                 };
                 auto step = [&](auto at_k) {
                     read(std::integral_constant<int, 0>(), at_k);
-                    if constexpr (S::kParts == 2) read(std::integral_constant<int, 1>(), at_k);
+                    if constexpr (S::kParts == 3) {
+                        read(std::integral_constant<int, 1>(), at_k);
+                        read(std::integral_constant<int, 2>(), at_k);
+                    }
                     if constexpr (S::kParts > 1 || PL == kAlongK) multiply<S::kParts>(acc, fp, fq, 0, S::FN);
                     if (SUMS != kNoSums) {
-                        const uint32_t one = S::kParts == 2 ? 0x3c003c00u : 0x3f803f80u;      // two ones
+                        const uint32_t one = 0x3f803f80u;      // two bfloat16 ones
                         const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one, one, one, one});
 #pragma unroll
                         for (int s = S::kParts - 1; s >= 0; s--)
 #pragma unroll
                             for (int i = 0; i < kSums; i++)
                                 sums[i] = SUMS == kSumP
-                                              ? mma(fp[s][i], ones, sums[i])
-                                              : mma(ones, fq[s][i], sums[i]);
+                                              ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[s][i], ones, sums[i], 0, 0, 0)
+                                              : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fq[s][i], sums[i], 0, 0, 0);
                     }
                 };
                 step(std::integral_constant<int, 0>());

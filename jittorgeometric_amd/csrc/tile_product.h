@@ -12,8 +12,8 @@
 // bfloat16 enters v_mfma_f32_16x16x32_bf16 as it is.  A float is split into three bfloat16 parts
 // a = a1 + a2 + a3, each the remainder rounded to 8 bits, which together hold its 24 bits; six of
 // the nine products of parts are summed in fp32 (a1b1, a1b2, a2b1, a1b3, a2b2, a3b1).  The parts are
-// at most 2^-9 and 2^-18 of a, so the dropped products are under 2^-26 of a * b: below the rounding
-// of the fp32 sums.  Six bfloat16 steps cost 6 / 16 of the fp32 matrix instruction's time on this
+// at most 2^-8 and 2^-17 of a, so the dropped products (a2b3, a3b2, a3b3) are under 2^-23.9 of a * b: about
+// one rounding of a float, which each of the fp32 sums has too.  Six bfloat16 steps cost 6 / 16 of the fp32 matrix instruction's time on this
 // chip (2.5 PFLOP/s against 157 TFLOP/s).  Floats of 2^128 (1 - 2^-9) and beyond, infinities and NaN
 // have no such parts: results they enter are NaN.
 #pragma once
@@ -71,7 +71,6 @@ template <> struct Eight<bf16> {
     }
     __device__ __forceinline__ void clear() { v = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void store(char *lds, int) const { *reinterpret_cast<u32x4 *>(lds) = v; }
-    __device__ __forceinline__ void store_parts(bf16 *out, int64_t) const { *reinterpret_cast<u32x4 *>(out) = v; }
     __device__ __forceinline__ void scale(float g)      // zero makes zero of anything
     {
 #pragma unroll

@@ -139,12 +139,12 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
     the loss is float32.  A class may be masked with a bias of -inf.  What a row without a label holds
     does not matter.
 
-    Products are summed in float32.  float32 entries keep 24 bits down to 2^-17 of the largest of
-    their array and 2^-39 of that largest below; an infinity or a NaN makes the logits it enters NaN or
-    infinite.
-    The gradient of the logits is rounded to bfloat16 on its way into the other gradients, or, in
-    float32, held to 24 bits and at least 2^-40.  The scratch memory of a backward pass is up to a
-    gigabyte of those, float32 sums of the size of weight, and one or two copies of x."""
+    Products are summed in float32.  float32 entries, and float32 gradients of the logits, keep their 24
+    bits (from 2^-103 on; below, an absolute 2^-126); an infinity or a NaN makes the logits it enters NaN or
+    infinite.  In bfloat16 the gradient of the logits is rounded to bfloat16 on its way into the other
+    gradients, and with reduction="none" so are the rows of x times their own gradient.  The scratch
+    memory of a backward pass is up to a gigabyte of gradients of logits, float32 sums of the size of
+    weight, and, in float32 one and a half times their size each, copies of x and weight."""
     _lib.require_gpu(x, weight, target, bias)
     if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
         raise _lib.JgamdError("linear_cross_entropy: x must be [rows, features] and weight [classes, features], got %s "
