@@ -7,13 +7,13 @@
 // Without y this is the first norm of a network: s = x.  Every array may be float or bfloat16;
 // everything between the loads and the stores is fp32, h is taken from s before s is rounded.
 //
-// Backward, with t = ds + rs (dh w), q = scale sigmoid(gate) and means over f:
-//     dx = t - s rs^3 mean(dh w s)                          (= the whole gradient of s)
-//     dy = ry dx q post - y ry^3 mean(dx q post y),  dgate = dx q (y ry post) (1 - sigmoid(gate))
+// Backward, with t = ds + rs (dh w), z = q post (y ry), q = scale sigmoid(gate) and means over f:
+//     dx = t - (s rs) rs m,   m = mean(dh w s) rs           (= the whole gradient of s)
+//     dy = ry dx q post - (y ry) ry mean(dx z),   dgate = dx q (y ry post) (1 - sigmoid(gate))
 //     dw = sum_r dh s rs,   dpost = sum_r dx q y ry,   dscale = sum_r dx sigmoid(gate) y ry post
-// The second mean needs dx, which needs the first; written out, mean(dx q post y) =
-// mean(t q post y) - rs^3 mean(dh w s) mean(s q post y), so that one reduction of three sums over
-// the row serves both.  s is recomputed from x, y, gate (read anyway) with the two inverse norms
+// The second mean needs dx, which needs the first; written out, mean(dx z) = mean(t z) - rs m rs mean(s z),
+// so that one reduction of three sums over the row serves both.  Every inverse norm stands at a factor
+// of its row's size: rs^3 by itself leaves float32 for rows of 1e13 and of 1e-13.  s is recomputed from x, y, gate (read anyway) with the two inverse norms
 // that the forward leaves (8 bytes a row), not from its rounded copy.
 //
 // Bound by memory.  L lanes share a row (L the power of two that covers it with 16 bytes a lane, up
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
             next.ds[c].get(t[c]);
         }
         if (kAhead && row0 + stride < a.R) next = read(row + stride);
-        float sums[3] = {0.f, 0.f, 0.f};      // dh w s, t q post y, s q post y
+        float sums[3] = {0.f, 0.f, 0.f};      // dh w s, t z, s z
 #pragma unroll
         for (int c = 0; c < C; c++) {
             const Small k = kKeep ? kept[c] : small(c);
@@ -374,8 +374,8 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
             }
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float z = BLOCK ? k.scale[i] * g[c][i] * k.post[i] * b[c][i] : 0.f;
-                if (BLOCK) s[c][i] += z * ry;
+                const float z = BLOCK ? k.scale[i] * g[c][i] * k.post[i] * (b[c][i] * ry) : 0.f;
+                if (BLOCK) s[c][i] += z;
                 const float hw = e[c][i] * k.w[i];
                 t[c][i] += rs * hw;
                 sums[0] += hw * s[c][i];
@@ -388,8 +388,8 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
         }
         if (BLOCK) row_sum<L>(sums, scratch);
         else row_sum<L>(reinterpret_cast<float(&)[1]>(sums), scratch);
-        const float back = rs * rs * rs * (sums[0] * over_f);
-        const float back_y = post ? ry * ry * ry * ((sums[1] - back * sums[2]) * over_f) : 0.f;
+        const float back = rs * (sums[0] * rs * over_f);
+        const float back_y = post ? ry * ((sums[1] - back * (rs * sums[2])) * over_f) : 0.f;
 #pragma unroll
         for (int c = 0; c < C; c++) {
             const Small k = kKeep ? kept[c] : small(c);
@@ -397,11 +397,11 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
             float dy[V], dg[V];
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float dx = t[c][i] - s[c][i] * back;
+                const float dx = t[c][i] - (s[c][i] * rs) * back;
                 t[c][i] = dx;
                 if (!BLOCK) continue;
                 const float u = b[c][i] * ry, xg = dx * g[c][i], dv = xg * k.scale[i], up = u * k.post[i];
-                dy[i] = ry * (dv * k.post[i]) - b[c][i] * back_y;
+                dy[i] = ry * (dv * k.post[i]) - u * back_y;
                 dg[i] = dv * up * (1.f - g[c][i]);
                 sum_p[c][i] += dv * u;
                 sum_s[c][i] += xg * up;

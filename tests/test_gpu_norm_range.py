@@ -1,10 +1,59 @@
-"""nn.rms_norm on more rows than one dimension of a launch counts threads for."""
+"""nn.residual_norm and nn.rms_norm on rows far from one and on more rows than one
+dimension of a launch counts.  Formulas and tolerances are those of test_gpu_norm.py: every size there is
+an expression in the rows themselves, so that it follows them to any magnitude."""
 import pytest
 import torch
 
+import test_gpu_norm as norm
+from test_gpu_norm import check, inputs, reference, run
 from util import dev
 
 pytestmark = pytest.mark.gpu
+
+DTYPES = norm.DTYPES
+
+
+def scaled(t, rows, by):
+    with torch.no_grad():
+        for k, c in by.items():
+            if t[k] is not None:
+                t[k][rows] *= c
+    return t
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("options", ["", "pgk"])
+@pytest.mark.parametrize("by", [{"x": 1e15, "y": 1e15}, {"x": 1e17, "y": 1e17}, {"x": 1e17}, {"y": 1e17}, {"x": 1e-13, "y": 1e17}])
+def test_large_rows(by, options, dtype):
+    """Squares of 1e17 and their sums over a row of 256 are far inside float32's range."""
+    t, ds, dh = inputs(24, 256, dtype, options)
+    t = scaled(t, slice(3, 20), by)
+    got, want = run(t, ds, dh), reference(t, ds, dh)
+    for k in got:
+        check(got[k], want[k], 256, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("options", ["", "pgk"])
+@pytest.mark.parametrize("c", [1e-13, 1e-16])
+def test_small_rows_without_eps(c, options, dtype, monkeypatch):
+    monkeypatch.setattr(norm, "EPS", 0.0)
+    t, ds, dh = inputs(24, 256, dtype, options)
+    t = scaled(t, slice(None), {"x": c, "y": c, "scale": c} if options else {"x": c, "y": c})
+    got, want = run(t, ds, dh), reference(t, ds, dh)
+    for k in got:
+        check(got[k], want[k], 256, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c,eps", [(1e15, 1e-6), (1e17, 1e-6), (1e-13, 0.0)])
+def test_rms_norm_of_large_and_small_rows(c, eps, dtype, monkeypatch):
+    monkeypatch.setattr(norm, "EPS", eps)
+    t, _, dh = inputs(30, 300, dtype, "", block=False)
+    t = scaled(t, slice(None), {"x": c})
+    got, want = run(t, None, dh), reference(t, None, dh)
+    for k in got:
+        check(got[k], want[k], 300, k)
 
 
 def test_more_rows_than_threads_in_one_dimension():
