@@ -9,7 +9,7 @@
 //
 // Backward, with t = ds + rs (dh w), z = q post (y ry), q = scale sigmoid(gate) and means over f:
 //     dx = t - (s rs) rs m,   m = mean(dh w s) rs           (= the whole gradient of s)
-//     dy = ry dx q post - (y ry) ry mean(dx z),   dgate = dx q (y ry post) (1 - sigmoid(gate))
+//     dy = ry dx q post - (y ry) ry mean(dx z),   dgate = dx q (y ry post) sigmoid(-gate)
 //     dw = sum_r dh s rs,   dpost = sum_r dx q y ry,   dscale = sum_r dx sigmoid(gate) y ry post
 // The second mean needs dx, which needs the first; written out, mean(dx z) = mean(t z) - rs m rs mean(s z),
 // so that one reduction of three sums over the row serves both.  Every inverse norm stands at a factor
@@ -174,6 +174,16 @@ struct NormArgs {
 
 // hardware exponential and reciprocal: within a few units of the last place
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+
+// The smaller of sigmoid(g) and sigmoid(-g), negative where it is the first: one register for both.  1 - sigmoid(g)
+// of a rounded sigmoid is off by 1 % at g = 12 and zero from 17 on.
+__device__ __forceinline__ float sigmoids(float g)
+{
+    const float e = __expf(-fabsf(g));
+    return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
+}
+__device__ __forceinline__ float open_of(float v) { return signbit(v) ? -v : 1.f - v; }      // sigmoid(g)
+__device__ __forceinline__ float shut_of(float v) { return signbit(v) ? 1.f + v : v; }       // sigmoid(-g)
 
 template <int L> constexpr int norm_threads() { return L > 256 ? L : 256; }
 
@@ -367,14 +377,14 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
             const Small k = kKeep ? kept[c] : small(c);
             if (gate) {      // never without a block
 #pragma unroll
-                for (int i = 0; i < V; i++) g[c][i] = sigmoid(g[c][i]);
+                for (int i = 0; i < V; i++) g[c][i] = sigmoids(g[c][i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < V; i++) g[c][i] = 1.f;
+                for (int i = 0; i < V; i++) g[c][i] = 0.f;      // open: 1
             }
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float z = BLOCK ? k.scale[i] * g[c][i] * k.post[i] * (b[c][i] * ry) : 0.f;
+                const float z = BLOCK ? k.scale[i] * open_of(g[c][i]) * k.post[i] * (b[c][i] * ry) : 0.f;
                 if (BLOCK) s[c][i] += z;
                 const float hw = e[c][i] * k.w[i];
                 t[c][i] += rs * hw;
@@ -400,9 +410,9 @@ __global__ __launch_bounds__(norm_threads<L>(), C == 1 ? 4 : 2) void norm_bwd(No
                 const float dx = t[c][i] - (s[c][i] * rs) * back;
                 t[c][i] = dx;
                 if (!BLOCK) continue;
-                const float u = b[c][i] * ry, xg = dx * g[c][i], dv = xg * k.scale[i], up = u * k.post[i];
+                const float u = b[c][i] * ry, xg = dx * open_of(g[c][i]), dv = xg * k.scale[i], up = u * k.post[i];
                 dy[i] = ry * (dv * k.post[i]) - u * back_y;
-                dg[i] = dv * up * (1.f - g[c][i]);
+                dg[i] = dv * up * shut_of(g[c][i]);
                 sum_p[c][i] += dv * u;
                 sum_s[c][i] += xg * up;
             }

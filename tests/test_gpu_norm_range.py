@@ -1,4 +1,4 @@
-"""nn.residual_norm and nn.rms_norm on rows far from one and on more rows than one
+"""nn.residual_norm and nn.rms_norm on rows far from one, with open gates and on more rows than one
 dimension of a launch counts.  Formulas and tolerances are those of test_gpu_norm.py: every size there is
 an expression in the rows themselves, so that it follows them to any magnitude."""
 import pytest
@@ -54,6 +54,24 @@ def test_rms_norm_of_large_and_small_rows(c, eps, dtype, monkeypatch):
     got, want = run(t, None, dh), reference(t, None, dh)
     for k in got:
         check(got[k], want[k], 300, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("F", [72, 1001])
+def test_gradient_of_gates_far_open_and_far_shut(F, dtype):
+    """dgate = dv u sigmoid(-gate): its error is relative to that product, however small the last factor
+    is, times 1 + |gate| for the argument of the exponential."""
+    t, ds, dh = inputs(41, F, dtype, "pgk")
+    with torch.no_grad():
+        t["gate"].copy_(torch.linspace(-60, 60, 41)[:, None].expand(41, F))
+    got, want = run(t, ds, dh), reference(t, ds, dh)
+    gate, y, p, k = (t[n].detach().double().cpu() for n in ("gate", "y", "post", "scale"))
+    shut = torch.sigmoid(-gate)
+    u = y / torch.sqrt((y * y).mean(1, keepdim=True) + norm.EPS) * p
+    dv = want["dx"][0] * k * torch.sigmoid(gate)
+    check(got["dgate"], (dv * u * shut, want["dgate"][1] * shut, 0), F, "dgate")
+    for name in ("s", "h", "dx", "dy"):
+        check(got[name], want[name], F, name)
 
 
 def test_more_rows_than_threads_in_one_dimension():
