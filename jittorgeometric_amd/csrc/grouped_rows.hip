@@ -615,10 +615,13 @@ template <typename T, typename S, Layout WL> static int32_t launch_rows(const Gr
 // against 256).  169343 rows of 200 floats to 129: 175 us with two tiles of 128, 142 with three of 64.
 static bool narrow_tiles(int n) { return ceil_div(n, 64) * 64 * 4 <= ceil_div(n, 128) * 128 * 3; }
 
-// workgroups of a streaming launch: those resident at once, more only if one had over kRunsKept tiles
+// Workgroups of a streaming launch: those resident at once, more only if one had over kRunsKept tiles.  Beside the
+// stages LDS holds the runs: tiles of 64 columns, two of whose 80 KB would fill a compute unit, have one workgroup
+// on each (120000 rows, 256 -> 64: 18.0 us, 20.7 with a grid for two; 60000 rows, 1024 x 64, dW: 70 and 74)
 template <typename S> static unsigned stream_grid(int64_t tiles)
 {
-    const int64_t resident = 256 * (160 * 1024 / S::kLds);
+    constexpr int kRunBytes = kRunsKept * (int)sizeof(Run) + S::kWaves * (int)sizeof(int);
+    const int64_t resident = 256 * (160 * 1024 / (S::kLds + kRunBytes));
     return (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(resident, ceil_div(ceil_div(tiles, kRunsKept), 8) * 8));
 }
 // 256 x 128 results (two workgroups a compute unit, steps of 32) against 256 x 256 (one, steps of 64): 65521 rows,

@@ -74,14 +74,15 @@ template <int OFFSET, int LINE> __device__ __forceinline__ void fragments_across
         out[i] = __builtin_bit_cast(bf16x8, u32x4{v[2 * i][0], v[2 * i][1], v[2 * i + 1][0], v[2 * i + 1][1]});
 }
 
-// Widths of tiles for an n that is a fraction of 256: 64 (two workgroups a compute unit), 128, 256.  The
-// fewer n a tile has, the more of its time goes into loading Q: a column of a tile of 128 is taken to
-// cost 1.1, of 64 1.25 of one of 256.
+// Widths of tiles for an n that is a fraction of 256.  The fewer n a tile has, the more of its time goes into
+// loading Q: a column of a tile of 128 is taken to cost 1.1 of one of 256, and tiles of 64 are for an n of up to 64
+// (typed, 120000 rows, 256 -> 64 bfloat16: 18.0 us, 20.6 in tiles of 128; n = 192 in three tiles of 64 or one of 256:
+// typed, 60000 rows of 1024: 46 and 37 us, class head, 8000 rows, 20000 classes, training: floats 1.96 and 1.71 ms,
+// bfloat16 495 and 460 us; n = 320 in five of 64 or three of 128: 52 and 45 us, 2.99 and 2.56 ms, 727 and 686 us).
 inline int stream_width(int64_t n)
 {
-    const double full = (double)((n + 255) / 256 * 256), half = 1.1 * (double)((n + 127) / 128 * 128),
-                 quarter = 1.25 * (double)((n + 63) / 64 * 64);
-    return quarter <= half && quarter <= full ? 64 : half <= full ? 128 : 256;
+    const double full = (double)((n + 255) / 256 * 256), half = 1.1 * (double)((n + 127) / 128 * 128);
+    return n <= 64 ? 64 : half <= full ? 128 : 256;
 }
 template <int PARTS, int WIDTH, int STEP> struct StreamOfWidth;
 template <int PARTS, int STEP> struct StreamOfWidth<PARTS, 256, STEP> {
