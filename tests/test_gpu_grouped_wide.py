@@ -1,5 +1,6 @@
-"""The typed product in bfloat16 at widths next to those where other tiles take over, and with more
-tiles than a workgroup keeps.  Formulas and tolerances are those of test_gpu_grouped.py."""
+"""The typed product in bfloat16 in its widest tiles (256 x 256), over several steps of k, ragged ones,
+several tiles of columns and of rows a workgroup and several pieces of a weight gradient; and at widths
+next to those where narrower tiles take over.  Formulas and tolerances are those of test_gpu_grouped.py."""
 import pytest
 import torch
 
@@ -9,6 +10,19 @@ from util import dev
 pytestmark = pytest.mark.gpu
 
 SIZES = [23011, 0, 255, 256, 257, 9001, 1, 7300]
+
+
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("K,N", [(256, 256), (264, 512), (512, 248), (248, 264), (256, 200), (200, 1000), (520, 776)])
+def test_widest_tiles(K, N, bias):
+    x, w, b, dout = inputs(sum(SIZES) + 11, K, N, len(SIZES), torch.bfloat16, seed=K + N, bias=bias)
+    off = offsets_of(SIZES, start=5)
+    got, again, want = run(x, w, b, off, dout), run(x, w, b, off, dout), reference(x, w, b, off, dout)
+    for k in got:
+        check(got[k], want[k], k)
+        assert torch.equal(got[k], again[k]), k
+    for k in ("out", "dx"):
+        assert not got[k][:5].any() and not got[k][-6:].any()
 
 
 @pytest.mark.parametrize("K,N", [(64, 64), (64, 72), (72, 64), (56, 192), (192, 128), (136, 320), (320, 136), (64, 256), (1024, 64)])
