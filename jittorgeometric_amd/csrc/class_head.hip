@@ -128,9 +128,6 @@ __device__ __forceinline__ int tiles_of(int mtiles, int ntiles)
     return first < all ? (int)((all - 1 - first) / g + 1) : 0;
 }
 
-// the largest finite bfloat16
-constexpr float kBf16Max = 0x1.fep+127f;
-
 // eight neighbouring values as one or three bfloat16 parts, kept where `keep` has ones
 template <int PARTS> __device__ __forceinline__ void store_parts8(bf16 *out, int64_t part, float (&v)[8], uint32_t keep)
 {
@@ -195,19 +192,11 @@ template <typename T> __global__ __launch_bounds__(256) void head_parts(Copies a
     if (id >= c.R * (a.ld / 8)) return;
     const Eight<T> e = copy_piece<T>(a, c, id);
     if constexpr (sizeof(T) == 4) {
-        // the first part stays finite: past kBf16Max the second takes what is left.  An infinity gives
-        // infinity and NaN as the other two, a NaN (which the clamp makes a number) NaN.
-        float first[8], rest[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float v = i < 4 ? e.a[i & 3] : e.b[i & 3];
-            first[i] = fminf(fmaxf(v, -kBf16Max), kBf16Max);
-            rest[i] = v;
-        }
+        float rest[8] = {e.a[0], e.a[1], e.a[2], e.a[3], e.b[0], e.b[1], e.b[2], e.b[3]};
         u32x4 w;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            w[i] = pack_bf16(first[2 * i], first[2 * i + 1]);
+            w[i] = pack_bf16(finite(rest[2 * i]), finite(rest[2 * i + 1]));
             rest[2 * i] -= bf16_lo(w[i]);
             rest[2 * i + 1] -= bf16_hi(w[i]);
         }

@@ -14,8 +14,7 @@
 // the nine products of parts are summed in fp32 (a1b1, a1b2, a2b1, a1b3, a2b2, a3b1).  The parts are
 // at most 2^-8 and 2^-17 of a, so the dropped products (a2b3, a3b2, a3b3) are under 2^-23.9 of a * b: about
 // one rounding of a float, which each of the fp32 sums has too.  Six bfloat16 steps cost 6 / 16 of the fp32 matrix instruction's time on this
-// chip (2.5 PFLOP/s against 157 TFLOP/s).  Floats of 2^128 (1 - 2^-9) and beyond, infinities and NaN
-// have no such parts: results they enter are NaN.
+// chip (2.5 PFLOP/s against 157 TFLOP/s).  Infinities and NaN have no such parts: results they enter are NaN.
 #pragma once
 #include "common.h"
 
@@ -54,6 +53,11 @@ template <> __device__ __forceinline__ bf16 from_float<bf16>(float v)
 {
     return bf16{(uint16_t)__builtin_bit_cast(uint16_t, (__bf16)v)};
 }
+
+// What the first part of a float is rounded from: past the largest bfloat16 (3.39e38) that one, and the second
+// part takes the rest.  An infinity or a NaN gives something finite here and NaN as the last part.  60000 rows,
+// 512 x 500 floats, forward: 201 us without it, 205 with it.
+__device__ __forceinline__ float finite(float v) { return __builtin_amdgcn_fmed3f(v, -0x1.fep+127f, 0x1.fep+127f); }
 
 // eight elements on their way from memory to LDS
 template <typename T> struct Eight;
@@ -107,7 +111,7 @@ template <> struct Eight<float> {
             u32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                w[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+                w[i] = s == 0 ? pack_bf16(finite(r[2 * i]), finite(r[2 * i + 1])) : pack_bf16(r[2 * i], r[2 * i + 1]);
                 r[2 * i] -= bf16_lo(w[i]);
                 r[2 * i + 1] -= bf16_hi(w[i]);
             }

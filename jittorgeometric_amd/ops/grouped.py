@@ -59,8 +59,9 @@ def grouped_rows(x, weight, offsets, bias=None):
     offsets [types + 1], integers on the GPU, where they stay: nothing waits for the device.  Rows of
     no type (before offsets[0], from offsets[types] on) give zero rows and get zero gradients; a type
     may have no rows.  Offsets that fall or leave [0, rows] are read as their running maximum clamped
-    to that range.  Sums are held in float32; a float32 product keeps float32's 24 bits, but an entry
-    of 3.39e38 or more, an infinity or a NaN makes the results it enters NaN."""
+    to that range.  Sums are held in float32; a float32 product keeps float32's 24 bits (of entries from
+    2^-103 on; below, an absolute 2^-126).  An infinity or a NaN makes the results it enters infinite or NaN:
+    in float32 NaN, except where few rows read the weights on the vector unit."""
     _lib.require_gpu(x, weight, offsets, bias)
     if x.dim() != 2 or weight.dim() != 3 or weight.shape[1] != x.shape[1]:
         raise _lib.JgamdError("grouped_rows: x must be [rows, Fin] and weight [types, Fin, Fout], got %s and %s"
