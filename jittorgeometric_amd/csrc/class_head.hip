@@ -313,7 +313,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void head_stats(HeadArgs a, int ran
 // lane one class of two rows, whose running maximum and sum it keeps.  Bound by reading w for up to kThinRows
 // rows, by the vector unit beyond.  Whole calls, with parts and like this: 4 rows, 387 features, 48749 classes 66
 // and 26 us; 256 features, 50021 classes: 7 rows 48 and 24, 24 rows 47 and 45, 32 rows 48 and 46, 48 rows 49 and 65;
-// 2000 features, 20000 classes, 32 rows: 193 and 157.  (bfloat16 of odd widths, copied once: 8 rows 23 and 27, 32 rows 23 and 46.)
+// 2000 features, 20000 classes, 32 rows: 193 and 157.  (bfloat16 of odd widths, copied once: 8 rows 23 and 27, 32 rows
+// 23 and 46.)
 // grid: x = blocks of kThinRows rows x ranges of tiles of 64 classes
 constexpr int kThinRows = 8;
 constexpr int kThinMost = 32;            // rows of a call, at most
@@ -852,7 +853,8 @@ template <typename T> struct HeadScratch {      // of the forward pass, then of 
     }
     size_t bytes() const
     {
-        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(gx, 2) + carve_bytes(scale, 4) + carve_bytes(stats, 8) + carve_bytes(at_label, 4) +
+        return carve_bytes(x, 2) + carve_bytes(w, 2) + carve_bytes(gx, 2) + carve_bytes(scale, 4) + carve_bytes(stats, 8) +
+               carve_bytes(at_label, 4) +
                carve_bytes(blocks, 8) + carve_bytes(blocks, 4) + carve_bytes(d, 2) + carve_bytes(part, 4) +
                carve_bytes(part_b, 4) + carve_bytes(acc_x, 4) + carve_bytes(acc_w, 4) + carve_bytes(acc_b, 4);
     }
@@ -892,7 +894,8 @@ static int32_t head_operands(HeadArgs *h, const void *x, const void *w, bf16 *xs
     h->x = xs;
     h->w = ws;
     const int64_t blocks = ceil_div(h->part_x / 8, 256) + ceil_div(h->part_w / 8, 256);
-    if (blocks > 0x7fffffffLL) return fail(JGAMD_ERR_SIZE, "linear_cross_entropy: V=%lld F=%d C=%d is too large", (long long)h->V, h->F, h->C);
+    if (blocks > 0x7fffffffLL)
+        return fail(JGAMD_ERR_SIZE, "linear_cross_entropy: V=%lld F=%d C=%d is too large", (long long)h->V, h->F, h->C);
     const Copy of[2] = {{x, nullptr, 1, h->V, xs, h->part_x}, {w, nullptr, 0, h->C, ws, h->part_w}};
     head_copies<T>(of, 2, *h, s);
     return launch_status("linear_cross_entropy");

@@ -13,8 +13,8 @@
 //     dw = sum_r dh s rs,   dpost = sum_r dx q y ry,   dscale = sum_r dx sigmoid(gate) y ry post
 // The second mean needs dx, which needs the first; written out, mean(dx z) = mean(t z) - rs m rs mean(s z),
 // so that one reduction of three sums over the row serves both.  Every inverse norm stands at a factor
-// of its row's size: rs^3 by itself leaves float32 for rows of 1e13 and of 1e-13.  s is recomputed from x, y, gate (read anyway) with the two inverse norms
-// that the forward leaves (8 bytes a row), not from its rounded copy.
+// of its row's size: rs^3 by itself leaves float32 for rows of 1e13 and of 1e-13.  s is recomputed from x, y,
+// gate (read anyway) with the two inverse norms that the forward leaves (8 bytes a row), not from its rounded copy.
 //
 // Bound by memory.  L lanes share a row (L the power of two that covers it with 16 bytes a lane, up
 // to a whole workgroup), the row stays in registers between the reduction and the stores.  A

@@ -10,8 +10,8 @@
 // descriptor's range, which the hardware answers with zeros: k past the end adds nothing.  Rows past
 // the last of a tile repeat a row that exists and are not stored.
 //
-// The LDS image is in lines of 32 or 64 k, or of the tile's rows: a wavefront's load writes 1 KB in lane order, so the
-// permutation is applied to the address each lane asks for.
+// The LDS image is in lines of 32 or 64 k, or of the tile's rows: a wavefront's load writes 1 KB in lane
+// order, so the permutation is applied to the address each lane asks for.
 //
 // Which row of P stands at which row of a 16 x 16 fragment is free.  In pairs the fragments 2 i and
 // 2 i + 1 of a wavefront share 32 rows such that a lane's two times four results are eight
@@ -42,7 +42,8 @@ template <int PARTS, int BN_, int BM_, int WN_, int WM_, int STEP_, int STAGES_>
     static_assert(PARTS == 1 || PARTS == 3, "of a bfloat16 or of a float");
     static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
     static constexpr int FN = BN / WN / 16, FM = BM / WM / 16;
-    static constexpr int kLoadsP = BN * kStep / 512 / kWaves, kLoadsQ = BM * kStep / 512 / kWaves;      // of a wavefront, step and part
+    // of a wavefront, step and part
+    static constexpr int kLoadsP = BN * kStep / 512 / kWaves, kLoadsQ = BM * kStep / 512 / kWaves;
     static constexpr int kLoads = (kLoadsP + kLoadsQ) * PARTS;
     static constexpr int kPartP = BN * kStep * 2, kPartQ = BM * kStep * 2;
     static constexpr int kStage = (kPartP + kPartQ) * PARTS;
@@ -255,7 +256,8 @@ template <typename S, Layout PL, Layout QL, bool PAIRS = PL == kAlongK> struct S
             across_p[i] = lds_at + Place<S::BN, S::kStep, kAcrossK>::at(
                                        kPairs ? wn + (i >> 1) * 32 + 2 * line_row + (i & 1) * 4 : wn + 16 * i + line_row, line_k);
 #pragma unroll
-        for (int j = 0; j < S::FM; j++) across_q[j] = lds_at + S::kParts * S::kPartP + Place<S::BM, S::kStep, kAcrossK>::at(wm + 16 * j + line_row, line_k);
+        for (int j = 0; j < S::FM; j++)
+            across_q[j] = lds_at + S::kParts * S::kPartP + Place<S::BM, S::kStep, kAcrossK>::at(wm + 16 * j + line_row, line_k);
         int stage_at = 0;
         for (int t = 0; t < tiles; t++) {
             f32x4 acc[S::FN][S::FM], sums[kSums];

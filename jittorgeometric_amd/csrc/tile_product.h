@@ -13,8 +13,9 @@
 // a = a1 + a2 + a3, each the remainder rounded to 8 bits, which together hold its 24 bits; six of
 // the nine products of parts are summed in fp32 (a1b1, a1b2, a2b1, a1b3, a2b2, a3b1).  The parts are
 // at most 2^-8 and 2^-17 of a, so the dropped products (a2b3, a3b2, a3b3) are under 2^-23.9 of a * b: about
-// one rounding of a float, which each of the fp32 sums has too.  Six bfloat16 steps cost 6 / 16 of the fp32 matrix instruction's time on this
-// chip (2.5 PFLOP/s against 157 TFLOP/s).  Infinities and NaN have no such parts: results they enter are NaN.
+// one rounding of a float, which each of the fp32 sums has too.  Six bfloat16 steps cost 6 / 16 of the fp32
+// matrix instruction's time on this chip (2.5 PFLOP/s against 157 TFLOP/s).  Infinities and NaN have no such
+// parts: results they enter are NaN.
 #pragma once
 #include "common.h"
 
